@@ -160,4 +160,69 @@ cudaError_t launch_copy_probe(void* dst, const void* src, long long bytes, int c
 cudaError_t launch_reduce_probe(void* dst, const void* const* srcs, int k, long long bytes, int ctas, int threads,
                                 cudaStream_t stream);
 
+// Mixture-of-experts operators around an AllToAll (experts.cu, int4.cu).  T tokens, E experts, k choices per
+// token; an assignment is one (token, choice) pair, numbered t * k + j.  Row strides are in elements.
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxChoices = 32;
+
+struct RouteArgs {
+  const void* logits;        // [T, E], rows logits_stride apart
+  long long logits_stride, tokens;
+  int dtype, experts, k;
+  int renormalize;           // 1: softmax over the chosen logits, 0: their share of the softmax over all
+  int* ids;                  // [T, k] chosen experts, -1 where no finite logit is left
+  float* weights;            // [T, k]
+  const float* grad_weights; // [T, k] (backward)
+  void* grad_logits;         // [T, E] contiguous (backward)
+};
+cudaError_t launch_route(const RouteArgs& args, cudaStream_t stream);
+cudaError_t launch_route_backward(const RouteArgs& args, cudaStream_t stream);
+
+struct SortArgs {
+  const void* ids;           // [assignments]; a value outside [0, experts) has no row
+  int ids64;                 // ids are int64 (else int32)
+  long long assignments, rows;
+  int experts;
+  long long capacity;        // rows per expert; 0: every assignment is kept, experts are packed one after another
+  int* slot;                 // [assignments] row of the assignment or -1
+  int* source;               // [rows] assignment of the row or -1
+  int* counts;               // [experts] rows in use
+  int* starts;               // [experts] first row
+};
+cudaError_t launch_sort(const SortArgs& args, cudaStream_t stream);
+
+// dispatch: rows[slot] = tokens[t]; its gradient: tokens[t] = sum_j rows[slot]; combine: with weights; the
+// gradient of combine: rows[slot] = w * tokens[t], grad_weights = <tokens[t], saved rows[slot]>.
+struct ExchangeRowsArgs {
+  const void* in;            // the tensor read: tokens (dispatch, combine gradient) or rows
+  void* out;                 // the tensor written
+  const void* saved;         // combine gradient: the rows of the forward pass
+  long long in_stride, out_stride, saved_stride;
+  const int* slot;           // [T, k]
+  const int* source;         // [rows]
+  const float* weights;      // [T, k] (combine and its gradient)
+  float* grad_weights;       // [T, k] (combine gradient)
+  long long tokens, rows, hidden;
+  int k, dtype;
+};
+cudaError_t launch_dispatch(const ExchangeRowsArgs& args, cudaStream_t stream);
+cudaError_t launch_combine(const ExchangeRowsArgs& args, cudaStream_t stream);           // weights may be nullptr (1)
+cudaError_t launch_combine_backward(const ExchangeRowsArgs& args, cudaStream_t stream);
+
+struct Int4Args {
+  const void* x;             // [rows, inner]
+  long long x_stride, rows;
+  const int* starts;         // [segments] first row
+  const int* counts;         // [segments] rows
+  int segments, experts;     // segment s belongs to expert s % experts
+  const unsigned char* packed;  // [experts, n, inner / 2], the even inner index in the low half of a byte
+  const void* scales;        // [experts, n, inner / group]
+  int scales_fp32;           // scales are fp32 (else of x's dtype)
+  long long n, inner;
+  int group, dtype;
+  void* out;                 // [rows, n], rows out_stride apart
+  long long out_stride;
+};
+cudaError_t launch_int4_product(const Int4Args& args, cudaStream_t stream);
+
 }  // namespace vb

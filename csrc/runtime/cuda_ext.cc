@@ -332,8 +332,11 @@ class DevicePlan {
 
 }  // namespace
 
+void bind_experts(py::module_& m);   // experts_ext.cc
+
 PYBIND11_MODULE(_vbcuda, m) {
   m.doc() = "vericcl_b200 CUDA runtime: symmetric heap, schedule interpreter, helper kernels";
+  bind_experts(m);
   py::class_<Heap>(m, "Heap")
       .def(py::init<int, int, int, size_t, const std::string&, bool>())
       .def("exchange", [](Heap& h, double t) { py::gil_scoped_release r; h.get().exchange(t); })

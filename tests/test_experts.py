@@ -1,0 +1,601 @@
+"""Mixture-of-experts operators: refusals and weight layout (CPU), numerics against 64-bit references (GPU)."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from vericcl_b200.errors import RuntimeFailure                    # noqa: E402
+from vericcl_b200.ops import experts as ex                        # noqa: E402
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def half_step(dtype):
+    """Largest relative error of one rounding to ``dtype``."""
+    return torch.finfo(dtype).eps / 2
+
+
+def close(got, want, magnitude, dtype, terms):
+    """|got - want| <= one rounding of the result + the fp32 sum's error: ``terms`` roundings of at most 2^-24 of
+    the sum of the terms' magnitudes (each of the products and partial sums is no larger), + the smallest
+    subnormal step of ``dtype``."""
+    err = (got.double() - want).abs()
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    bound = half_step(dtype) * want.abs() + (1 + half_step(dtype)) * terms * 2.0 ** -24 * magnitude + tiny
+    assert bool((err <= bound).all()), (err - bound).max().item()
+
+
+# -- refusals (no GPU needed: every check runs before the device is touched) ---------------------------------
+
+def _cpu_order(tokens=3, k=2, rows=6):
+    return ex.ExpertOrder(torch.zeros(tokens, k, dtype=torch.int32), torch.zeros(rows, dtype=torch.int32),
+                          torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("call", [
+    lambda: ex.route(torch.zeros(3), 1),
+    lambda: ex.route(torch.zeros(3, 4, dtype=torch.float64), 1),
+    lambda: ex.route(torch.zeros(3, 4), 0),
+    lambda: ex.route(torch.zeros(3, 4), 5),
+    lambda: ex.route(torch.zeros(3, 2000), 2),
+    lambda: ex.route(torch.zeros(3, 64), 33),
+    lambda: ex.route(torch.zeros(4, 3).t(), 1),
+    lambda: ex.route_backward(torch.zeros(3, 4), torch.zeros(3, 2, dtype=torch.int64), torch.zeros(3, 2),
+                              torch.zeros(3, 2)),
+    lambda: ex.route_backward(torch.zeros(3, 4), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2),
+                              torch.zeros(2, 2)),
+    lambda: ex.sort_by_expert(torch.zeros(3, 2), 4),
+    lambda: ex.sort_by_expert(torch.zeros(6, dtype=torch.int32), 4),
+    lambda: ex.sort_by_expert(torch.zeros(2, 3, dtype=torch.int32).t(), 4),
+    lambda: ex.sort_by_expert(torch.zeros(3, 2, dtype=torch.int32), 0),
+    lambda: ex.sort_by_expert(torch.zeros(3, 2, dtype=torch.int32), 1025),
+    lambda: ex.sort_by_expert(torch.zeros(3, 2, dtype=torch.int32), 4, capacity=0),
+    lambda: ex.sort_by_expert(torch.zeros(3, 2, dtype=torch.int32), 1024, capacity=1 << 21),
+    lambda: ex.sort_by_expert(torch.zeros(3, 0, dtype=torch.int32), 4),
+    lambda: ex.sort_by_expert(torch.zeros(3, 33, dtype=torch.int32), 4),
+    lambda: ex.dispatch(torch.zeros(4, 8), _cpu_order()),
+    lambda: ex.dispatch(torch.zeros(3, 8, dtype=torch.int32), _cpu_order()),
+    lambda: ex.dispatch(torch.zeros(8, 3).t(), _cpu_order()),
+    lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order(), out=torch.zeros(5, 8)),
+    lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order(), out=torch.zeros(6, 8, dtype=torch.float16)),
+    lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order(), out=torch.zeros(1, 8).expand(6, 8)),
+    lambda: ex.dispatch_backward(torch.zeros(5, 8), _cpu_order()),
+    lambda: ex.combine(torch.zeros(5, 8), torch.zeros(3, 2), _cpu_order()),
+    lambda: ex.combine(torch.zeros(6, 8), torch.zeros(3, 2, dtype=torch.bfloat16), _cpu_order()),
+    lambda: ex.combine(torch.zeros(6, 8), torch.zeros(2, 3), _cpu_order()),
+    lambda: ex.combine_backward(torch.zeros(3, 8), torch.zeros(6, 9), torch.zeros(3, 2), _cpu_order()),
+    lambda: ex.combine_backward(torch.zeros(3, 8), torch.zeros(6, 8, dtype=torch.float16), torch.zeros(3, 2),
+                                _cpu_order()),
+    lambda: ex.quantize_int4(torch.zeros(8)),
+    lambda: ex.quantize_int4(torch.zeros(8, 100), 32),
+    lambda: ex.quantize_int4(torch.zeros(8, 96), 48),
+    lambda: ex.quantize_int4(torch.zeros(8, 128), 128, scale_dtype=torch.float64),
+])
+def test_refusals(call):
+    with pytest.raises(RuntimeFailure):
+        call()
+
+
+def _product_args(**change):
+    args = dict(rows=torch.zeros(5, 128, dtype=torch.bfloat16), starts=torch.zeros(2, dtype=torch.int32),
+                counts=torch.zeros(2, dtype=torch.int32), packed=torch.zeros(2, 7, 64, dtype=torch.uint8),
+                scales=torch.zeros(2, 7, 1, dtype=torch.bfloat16))
+    args.update(change)
+    return args
+
+
+@pytest.mark.parametrize("change", [
+    dict(rows=torch.zeros(5, 128)), dict(rows=torch.zeros(5, 126, dtype=torch.bfloat16)),
+    dict(rows=torch.zeros(128, 5, dtype=torch.bfloat16).t()),
+    dict(starts=torch.zeros(3, dtype=torch.int32)), dict(starts=torch.zeros(2, dtype=torch.int64)),
+    dict(counts=torch.zeros(4, dtype=torch.int32)),
+    dict(starts=torch.zeros(3, dtype=torch.int32), counts=torch.zeros(3, dtype=torch.int32)),
+    dict(starts=torch.zeros(0, dtype=torch.int32), counts=torch.zeros(0, dtype=torch.int32)),
+    dict(starts=torch.zeros(1026, dtype=torch.int32), counts=torch.zeros(1026, dtype=torch.int32)),
+    dict(packed=torch.zeros(2, 7, 64, dtype=torch.int8)), dict(packed=torch.zeros(2, 7, 63, dtype=torch.uint8)),
+    dict(packed=torch.zeros(7, 2, 64, dtype=torch.uint8).transpose(0, 1)),
+    dict(packed=torch.zeros(2 * 7 * 64 + 1, dtype=torch.uint8)[1:].view(2, 7, 64)),
+    dict(scales=torch.zeros(2, 7, 1, dtype=torch.float16)), dict(scales=torch.zeros(2, 7, 3, dtype=torch.bfloat16)),
+    dict(scales=torch.zeros(2, 7, 8, dtype=torch.bfloat16)), dict(scales=torch.zeros(2, 7, 0, dtype=torch.bfloat16)),
+    dict(scales=torch.zeros(2, 8, 1, dtype=torch.bfloat16)),
+    dict(rows=torch.zeros(5, 128, dtype=torch.bfloat16, requires_grad=True)),
+    dict(out=torch.zeros(5, 8, dtype=torch.bfloat16)), dict(out=torch.zeros(5, 7, dtype=torch.float16)),
+])
+def test_product_refusals(change):
+    with pytest.raises(RuntimeFailure):
+        ex.expert_matmul_int4(**_product_args(**change))
+
+
+def test_cpu_tensors_are_refused():
+    for call in (lambda: ex.route(torch.zeros(3, 4), 2),
+                 lambda: ex.sort_by_expert(torch.zeros(3, 2, dtype=torch.int32), 4),
+                 lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order()),
+                 lambda: ex.combine(torch.zeros(6, 8), torch.zeros(3, 2), _cpu_order()),
+                 lambda: ex.expert_matmul_int4(**_product_args())):
+        with pytest.raises(RuntimeFailure, match="CUDA"):
+            call()
+
+
+def dequantized(packed, scales, group):
+    q = torch.stack([packed & 15, packed >> 4], -1).flatten(-2).double() - 8
+    return (q.unflatten(-1, (-1, group)) * scales.double()[..., None]).flatten(-2)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_int4_is_within_half_a_step(group, dtype):
+    g = torch.Generator().manual_seed(group)
+    w = torch.randn(3, 5, 256, generator=g).to(dtype)
+    w[0, 0] = 0
+    packed, scales = ex.quantize_int4(w, group)
+    assert packed.shape == (3, 5, 128) and packed.dtype == torch.uint8
+    assert scales.shape == (3, 5, 256 // group) and scales.dtype == dtype
+    back = dequantized(packed, scales, group)
+    step = scales.double().repeat_interleave(group, -1)
+    # half a step, plus what the largest magnitudes lose when the rounded scale is below magnitude / 7, plus the
+    # fp32 quotient's rounding (a quotient of up to 7 is off by 2^-24 relative)
+    bound = step * (0.5 + 7 * (half_step(dtype) + 2.0 ** -22))
+    assert bool(((back - w.double()).abs() <= bound).all())
+    assert bool((back[0, 0] == 0).all())
+
+
+# -- numerics -----------------------------------------------------------------------------------------------
+
+def cuda(seed=0):
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+def reference_route(logits, k, renormalize):
+    x = logits.double().cpu()
+    ids = torch.full((x.size(0), k), -1, dtype=torch.int32)
+    w = torch.zeros(x.size(0), k, dtype=torch.float64)
+    for t in range(x.size(0)):
+        row = x[t]
+        order = sorted((e for e in range(len(row)) if row[e] > -math.inf), key=lambda e: (-row[e].item(), e))[:k]
+        if not order:
+            continue
+        ids[t, :len(order)] = torch.tensor(order, dtype=torch.int32)
+        chosen = row[order]
+        total = chosen if renormalize else row[row > -math.inf]
+        w[t, :len(order)] = torch.exp(chosen - row.max()) / torch.exp(total - row.max()).sum()
+    return ids.cuda(), w.cuda()
+
+
+# exp is within 2 units in the last place for arguments of any size (2^-22 relative), its argument's difference is
+# rounded once (2^-24 of at most 2 max|l|), the sum adds log2(32) + 32 roundings and the quotient one
+def route_bound(logits):
+    fine = logits.double().masked_fill(~torch.isfinite(logits.double()), 0)
+    return 2.0 ** -24 * (2 * 2 * fine.abs().max().item() + 2 * 4 + 40)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("tokens,experts,k", [(1, 1, 1), (1, 128, 8), (9, 5, 5), (17, 33, 2), (64, 257, 32), (7, 1024, 9)])
+def test_route_matches_reference(dtype, renormalize, tokens, experts, k):
+    g = cuda(tokens + experts)
+    logits = normal(g, tokens, experts, dtype=dtype, scale=3.0)
+    ids, w = ex.route(logits, k, renormalize=renormalize)
+    want_ids, want = reference_route(logits, k, renormalize)
+    assert torch.equal(ids, want_ids)
+    assert bool(((w.double() - want).abs() <= route_bound(logits) * want + 1e-38).all())
+    grad = normal(g, tokens, k)
+    got = ex.route_backward(logits, ids, w, grad, renormalize=renormalize)
+    inner = (want * grad.double()).sum(1, keepdim=True)
+    if renormalize:
+        expect = torch.zeros(tokens, experts, dtype=torch.float64, device="cuda")
+        expect.scatter_(1, ids.long(), want * (grad.double() - inner))
+    else:
+        share = torch.softmax(logits.double(), 1)
+        expect = share * (torch.zeros_like(share).scatter_(1, ids.long(), grad.double()) - inner)
+    # each factor carries the weights' relative error, on magnitudes of at most w (|g| + sum w |g|)
+    size = grad.abs().max().item() * 2
+    bound = half_step(dtype) * expect.abs() + (4 * route_bound(logits) + 40 * 2.0 ** -24) * size * \
+        torch.softmax(logits.double(), 1).clamp(min=0 if not renormalize else 1) + \
+        torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert bool(((got.double() - expect).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_masks_ties_and_nan(renormalize):
+    cuda()
+    inf, nan, low = math.inf, math.nan, torch.finfo(torch.float32).min
+    logits = torch.tensor([[1.0, 1, 1, 1], [-inf, 2, -inf, -inf], [-inf] * 4, [low] * 4, [0.0, -0.0, -1, low],
+                           [nan, 1, 2, 0], [5, low, -inf, low]], device="cuda")
+    ids, w = ex.route(logits, 3, renormalize=renormalize)
+    assert ids.tolist() == [[0, 1, 2], [1, -1, -1], [-1, -1, -1], [0, 1, 2], [0, 1, 2], [2, 1, 3], [0, 1, 3]]
+    third, quarter = 1 / 3, 1 / 4
+    each = third if renormalize else quarter
+    assert torch.allclose(w[0], torch.full((3,), each, device="cuda"))
+    assert w[1].tolist() == [1, 0, 0] and w[2].tolist() == [0, 0, 0]
+    assert torch.allclose(w[3], torch.full((3,), each, device="cuda"))
+    assert bool(w[5].isnan().all()) and w[6].tolist() == [1, 0, 0]
+    grad = ex.route_backward(logits, ids, w, torch.ones_like(w), renormalize=renormalize)
+    assert bool((grad[[1, 2]] == 0).all()) and bool(grad[[0, 3, 4, 6]].isfinite().all())
+
+
+def reference_order(ids, experts, capacity):
+    flat = ids.reshape(-1).tolist()
+    buckets = [[a for a, e in enumerate(flat) if e == want] for want in range(experts)]
+    rows = experts * capacity if capacity else len(flat)
+    slot, source, starts, counts = [-1] * len(flat), [-1] * rows, [], []
+    at = 0
+    for e, bucket in enumerate(buckets):
+        start = e * capacity if capacity else at
+        kept = bucket[:capacity] if capacity else bucket
+        for i, a in enumerate(kept):
+            slot[a], source[start + i] = start + i, a
+        starts.append(start)
+        counts.append(len(kept))
+        at += len(bucket)
+    make = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
+    return make(slot).view(ids.shape), make(source), make(counts), make(starts)
+
+
+def random_ids(g, tokens, k, experts, dtype=torch.int32):
+    ids = torch.randint(-1, experts + 1, (tokens, k), device="cuda", generator=g).to(dtype)   # -1 and experts: none
+    return ids
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("tokens,k,experts,capacity", [
+    (0, 2, 4, None), (0, 2, 4, 3), (1, 1, 1, None), (1, 8, 64, None), (1, 8, 64, 2), (33, 3, 7, None), (33, 3, 7, 5),
+    (1000, 2, 1024, None), (4099, 6, 60, 300), (5000, 8, 3, None), (40000, 4, 256, None), (40000, 4, 256, 700)])
+def test_sort_is_stable_and_complete(dtype, tokens, k, experts, capacity):
+    g = cuda(tokens)
+    ids = random_ids(g, tokens, k, experts, dtype)
+    order = ex.sort_by_expert(ids, experts, capacity=capacity)
+    want = reference_order(ids.cpu(), experts, capacity)
+    for got, expect in zip((order.slot, order.source, order.counts, order.starts), want):
+        assert torch.equal(got, expect)
+    again = ex.sort_by_expert(ids, experts, capacity=capacity)
+    assert torch.equal(again.slot, order.slot)
+
+
+@pytest.mark.gpu
+def test_sort_all_on_one_expert_and_none_at_all():
+    cuda()
+    ids = torch.full((3000, 4), 5, dtype=torch.int32, device="cuda")
+    order = ex.sort_by_expert(ids, 9)
+    assert order.counts.tolist() == [0] * 5 + [12000] + [0] * 3
+    assert torch.equal(order.slot.view(-1), torch.arange(12000, dtype=torch.int32, device="cuda"))
+    order = ex.sort_by_expert(ids, 9, capacity=7)
+    assert order.counts.tolist() == [0] * 5 + [7] + [0] * 3 and int((order.slot >= 0).sum()) == 7
+    order = ex.sort_by_expert(torch.full_like(ids, -1), 9)
+    assert bool((order.slot == -1).all()) and bool((order.source == -1).all()) and int(order.counts.sum()) == 0
+
+
+CASES = [(1, 1, 1, None, 1), (1, 8, 64, None, 4096), (5, 2, 4, None, 7), (33, 3, 7, 5, 1030), (64, 8, 16, 40, 96),
+         (257, 4, 8, None, 2048), (1000, 6, 60, 90, 515)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,k,experts,capacity,hidden", CASES)
+def test_dispatch_and_combine_match_reference(dtype, tokens, k, experts, capacity, hidden):
+    g = cuda(hidden)
+    order = ex.sort_by_expert(random_ids(g, tokens, k, experts), experts, capacity=capacity)
+    slot, kept = order.slot.long(), order.slot >= 0
+    x = normal(g, tokens, hidden, dtype=dtype)
+    rows = ex.dispatch(x, order)
+    expect = torch.zeros(order.rows, hidden, dtype=dtype, device="cuda")
+    expect[slot[kept]] = x.repeat_interleave(k, 0).view(tokens, k, hidden)[kept]
+    assert torch.equal(rows, expect)
+
+    def gathered(r):
+        return torch.where(kept[..., None], r.double()[slot.clamp(min=0)], 0.0)
+
+    # rows nobody owns must not be read: NaN there may not reach a result
+    values = normal(g, order.rows, hidden, dtype=dtype)
+    values[order.source < 0] = math.nan
+    weights = normal(g, tokens, k)
+    parts = gathered(values)
+    close(ex.dispatch_backward(values, order), parts.sum(1), parts.abs().sum(1), dtype, k)
+    parts = parts * weights.double()[..., None]
+    close(ex.combine(values, weights, order), parts.sum(1), parts.abs().sum(1), dtype, 2 * k)
+
+    grad = normal(g, tokens, hidden, dtype=dtype)
+    grad_rows, grad_weights = ex.combine_backward(grad, values, weights, order)
+    expect = torch.zeros(order.rows, hidden, dtype=torch.float64, device="cuda")
+    expect[slot[kept]] = (grad.double()[:, None] * weights.double()[..., None])[kept]
+    close(grad_rows, expect, expect.abs(), dtype, 1)
+    parts = gathered(values) * grad.double()[:, None]
+    close(grad_weights, parts.sum(2), parts.abs().sum(2), torch.float32, hidden)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hidden,offset,pitch", [(64, 8, 96), (64, 1, 67), (66, 2, 72), (128, 3, 1024)])
+def test_strided_and_broadcast_rows(dtype, hidden, offset, pitch):
+    g = cuda(pitch)
+    order = ex.sort_by_expert(random_ids(g, 50, 3, 6), 6)
+    wide = normal(g, 150, pitch + offset, dtype=dtype)
+    view = wide[:50, offset:offset + hidden]
+    store = torch.full((order.rows, pitch + offset), 7.0, device="cuda").to(dtype)
+    rows = ex.dispatch(view, order, out=store[:, offset:offset + hidden])
+    assert torch.equal(rows, ex.dispatch(view.contiguous(), order))
+    assert bool((store[:, :offset] == 7).all()) and bool((store[:, offset + hidden:] == 7).all())
+    values, weights = wide[:, offset:offset + hidden], normal(g, 50, 3)
+    assert torch.equal(ex.combine(values, weights, order), ex.combine(values.contiguous(), weights, order))
+    grads = ex.combine_backward(view, values, weights, order, out=store[:, offset:offset + hidden])
+    plain = ex.combine_backward(view.contiguous(), values.contiguous(), weights, order)
+    assert torch.equal(grads[0], plain[0]) and torch.equal(grads[1], plain[1])
+    assert bool((store[:, :offset] == 7).all()) and bool((store[:, offset + hidden:] == 7).all())
+    one = wide[:1, offset:offset + hidden].expand(50, hidden)
+    assert torch.equal(ex.dispatch(one, order), ex.dispatch(one.contiguous(), order))
+
+
+@pytest.mark.gpu
+def test_no_tokens_and_no_columns():
+    cuda()
+    order = ex.sort_by_expert(torch.zeros(0, 2, dtype=torch.int32, device="cuda"), 4, capacity=3)
+    rows = ex.dispatch(torch.zeros(0, 8, device="cuda"), order)
+    assert rows.shape == (12, 8) and bool((rows == 0).all())
+    assert ex.combine(rows, torch.zeros(0, 2, device="cuda"), order).shape == (0, 8)
+    grad_rows, grad_weights = ex.combine_backward(torch.zeros(0, 8, device="cuda"), rows,
+                                                  torch.zeros(0, 2, device="cuda"), order)
+    assert bool((grad_rows == 0).all()) and grad_weights.shape == (0, 2)
+    order = ex.sort_by_expert(torch.zeros(3, 2, dtype=torch.int32, device="cuda"), 4)
+    empty = torch.zeros(3, 0, device="cuda")
+    assert ex.dispatch(empty, order).shape == (6, 0)
+    got = ex.combine_backward(empty, torch.zeros(6, 0, device="cuda"), torch.ones(3, 2, device="cuda"), order)
+    assert bool((got[1] == 0).all())
+    ids, w = ex.route(torch.zeros(0, 4, device="cuda"), 2)
+    assert ids.shape == (0, 2) and w.shape == (0, 2)
+
+
+@pytest.mark.gpu
+def test_a_user_made_order_is_kept_inside_its_rows():
+    """Slots beyond the rows are treated like assignments without a row."""
+    cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    order = ex.ExpertOrder(torch.tensor([[0, 99], [-7, 1]], **i32), torch.tensor([0, 3], **i32),
+                           torch.tensor([2], **i32), torch.tensor([0], **i32))
+    x = torch.tensor([[1.0, 2], [3, 4]], device="cuda")
+    assert ex.dispatch(x, order).tolist() == [[1, 2], [3, 4]]
+    w = torch.full((2, 2), 2.0, device="cuda")
+    assert ex.combine(x, w, order).tolist() == [[2, 4], [6, 8]]
+    grad_rows, grad_weights = ex.combine_backward(x, x, w, order)
+    assert grad_rows.tolist() == [[2, 4], [6, 8]] and grad_weights.tolist() == [[5, 0], [0, 25]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_autograd_agrees_with_the_plain_calls(dtype, renormalize):
+    g = cuda(3)
+    logits = normal(g, 40, 12, dtype=dtype).requires_grad_()
+    x = normal(g, 40, 72, dtype=dtype).requires_grad_()
+    ids, w = ex.route(logits, 3, renormalize=renormalize)
+    order = ex.sort_by_expert(ids, 12, capacity=8)
+    rows = ex.dispatch(x, order)
+    y = ex.combine(rows * 2, w, order)
+    grad = normal(g, 40, 72, dtype=dtype)
+    y.backward(grad)
+    grad_rows, grad_w = ex.combine_backward(grad, rows.detach() * 2, w.detach(), order)
+    assert torch.equal(x.grad, ex.dispatch_backward(grad_rows * 2, order))
+    assert torch.equal(logits.grad, ex.route_backward(logits.detach(), ids, w.detach(), grad_w, renormalize=renormalize))
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    """Central differences in fp32: the functions are smooth, a step of 2^-6 leaves a relative error of about 2^-12
+    from the third derivative and 2^-24 * 2^6 * |loss| from the rounding of the loss."""
+    g = cuda(5)
+    logits, x = normal(g, 6, 5), normal(g, 6, 9)
+    ids, _ = ex.route(logits, 2)
+    order = ex.sort_by_expert(ids, 5)
+    up, mix = normal(g, 6, 9).double(), normal(g, 12, 9)
+
+    def loss(l, t):
+        # the choice is held: the gradient is that of the weights
+        p = torch.softmax(l.double(), 1).gather(1, ids.long()).float()
+        got = ex.combine(ex.dispatch(t, order) * mix, p, order)
+        return (got.double() * up).sum().item()
+
+    lg, xg = logits.clone().requires_grad_(), x.clone().requires_grad_()
+    got_ids, w = ex.route(lg, 2, renormalize=False)
+    assert torch.equal(got_ids, ids)
+    ex.combine(ex.dispatch(xg, order) * mix, w, order).backward(up.float())
+    h, size = 2.0 ** -6, (up.abs().sum() * 8).item()
+    for value, grad, which in ((logits, lg.grad, 0), (x, xg.grad, 1)):
+        for i in range(0, value.numel(), 4):
+            step = torch.zeros_like(value)
+            step.view(-1)[i] = h
+            pair = [(logits + s * step, x) if which == 0 else (logits, x + s * step) for s in (1, -1)]
+            difference = (loss(*pair[0]) - loss(*pair[1])) / (2 * h)
+            assert abs(difference - grad.view(-1)[i].item()) <= size * (2.0 ** -12 + 2.0 ** -24 * 2 ** 6)
+
+
+PRODUCTS = [(1, 1, 1, 1, 32, 32), (1, 64, 8, 64, 128, 64), (3, 4, 7, 33, 160, 32), (8, 64, 8, 256, 512, 128),
+            (17, 3, 17, 100, 384, 128), (37, 16, 13, 131, 2080, 32), (40, 2, 2, 16, 4096, 64), (100, 5, 4, 515, 896, 128),
+            (300, 2, 2, 130, 192, 64)]
+
+
+def product_case(g, rows, experts, active, n, inner, group, dtype, scale_dtype):
+    counts = torch.zeros(experts, dtype=torch.int64)
+    pick = torch.randint(0, min(active, experts), (rows,), generator=torch.Generator().manual_seed(rows))
+    chosen = torch.randperm(experts, generator=torch.Generator().manual_seed(n))[:min(active, experts)]
+    counts.scatter_add_(0, chosen[pick], torch.ones(rows, dtype=torch.int64))
+    starts = counts.cumsum(0) - counts
+    x = normal(g, rows, inner, dtype=dtype)
+    packed = torch.randint(0, 256, (experts, n, inner // 2), dtype=torch.uint8, device="cuda", generator=g)
+    scales = (0.01 + 0.02 * torch.rand(experts, n, inner // group, device="cuda", generator=g)).to(scale_dtype)
+    return x, starts.int().cuda(), counts.int().cuda(), packed, scales
+
+
+def product_reference(x, starts, counts, packed, scales, group):
+    """(values, sums of magnitudes) in 64 bits."""
+    out = torch.zeros(x.size(0), packed.size(1), dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(out)
+    for s, (at, c) in enumerate(zip(starts.tolist(), counts.tolist())):
+        w = dequantized(packed[s % packed.size(0)], scales[s % packed.size(0)], group)
+        out[at:at + c] = x[at:at + c].double() @ w.T
+        size[at:at + c] = x[at:at + c].double().abs() @ w.abs().T
+    return out, size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("wide_scales", [False, True])
+@pytest.mark.parametrize("rows,experts,active,n,inner,group", PRODUCTS)
+def test_int4_product_matches_reference(dtype, wide_scales, rows, experts, active, n, inner, group):
+    g = cuda(inner + n)
+    args = product_case(g, rows, experts, active, n, inner, group, dtype, torch.float32 if wide_scales else dtype)
+    want, size = product_reference(*args, group)
+    got = ex.expert_matmul_int4(*args)
+    # products and partial sums: at most inner additions, each of them and each group's scaling off by 2^-23 (the
+    # matrix unit may cut instead of rounding)
+    close(got, want, size, dtype, 2 * (inner + 3 * inner // group))
+    # that bound is the worst case; the fp32 errors have random signs, so over all outputs they stay near the error
+    # of one rounding of values as large as the partial sums (32 of which is 2^-19), far under the result's rounding
+    assert (got.double() - want).norm() <= (half_step(dtype) + 2.0 ** -16) * want.norm()
+    assert torch.equal(got, ex.expert_matmul_int4(*args))
+
+
+@pytest.mark.gpu
+def test_int4_product_segments_gaps_and_views():
+    """Segments of two source ranks, rows between them that no segment covers, strided rows and outputs."""
+    g = cuda(11)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    starts, counts = torch.tensor([0, 4, 8, 12], **i32), torch.tensor([3, 0, 4, 2], **i32)
+    _, _, _, packed, scales = product_case(g, 4, 2, 2, 50, 128, 64, torch.bfloat16, torch.bfloat16)
+    wide = normal(g, 17, 200, dtype=torch.bfloat16)
+    x = wide[:, 3:131]
+    store = torch.full((17, 60), 7.0, device="cuda", dtype=torch.bfloat16)
+    got = ex.expert_matmul_int4(x, starts, counts, packed, scales, out=store[:, 5:55])
+    want, size = product_reference(x, starts, counts, packed, scales, 64)
+    close(got, want, size, torch.bfloat16, 2 * (128 + 6))
+    for r in (3, 4, 5, 6, 7, 14, 15, 16):
+        assert bool((got[r] == 0).all())
+    assert bool((store[:, :5] == 7).all()) and bool((store[:, 55:] == 7).all())
+    none = ex.expert_matmul_int4(x, starts, torch.zeros_like(counts), packed, scales)
+    assert bool((none == 0).all())
+    assert ex.expert_matmul_int4(x[:0], starts, counts, packed, scales).shape == (0, 50)
+
+
+@pytest.mark.gpu
+def test_int4_product_keeps_segments_inside_the_rows():
+    g = cuda(12)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    _, _, _, packed, scales = product_case(g, 4, 2, 2, 20, 64, 32, torch.float16, torch.float16)
+    x = normal(g, 6, 64, dtype=torch.float16)
+    got = ex.expert_matmul_int4(x, torch.tensor([-3, 4], **i32), torch.tensor([5, 1000], **i32), packed, scales)
+    want, size = product_reference(x, torch.tensor([0, 4]), torch.tensor([2, 2]), packed, scales, 32)
+    close(got, want, size, torch.float16, 2 * (64 + 6))
+
+
+@pytest.mark.gpu
+def test_int4_product_infinities_and_nan_follow_the_formula():
+    cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q = torch.full((1, 3, 64), 8, dtype=torch.uint8, device="cuda")
+    q[0, 0, 5], q[0, 1, 5] = 11, 2                       # +3, -6 and (row 2) 0 times infinity
+    packed = q[..., 0::2] | (q[..., 1::2] << 4)
+    scales = torch.ones(1, 3, 2, device="cuda", dtype=torch.bfloat16)
+    x = torch.zeros(2, 64, device="cuda", dtype=torch.bfloat16)
+    x[0, 5] = math.inf
+    got = ex.expert_matmul_int4(x, torch.zeros(1, **i32), torch.full((1,), 2, **i32), packed, scales)
+    assert got[0, 0] == math.inf and got[0, 1] == -math.inf and bool(got[0, 2].isnan())
+    assert bool((got[1] == 0).all())
+
+
+@pytest.mark.gpu
+def test_the_set_together_eager_and_replayed_on_a_side_stream():
+    """Router, sort, dispatch, two 4-bit products and combine, as a serving step calls them; the captured step on
+    new inputs equals the eager one bit for bit."""
+    g = cuda(21)
+    tokens, experts, k, hidden, inner = 13, 8, 2, 256, 384
+    up = ex.quantize_int4(normal(g, experts, inner, hidden, dtype=torch.bfloat16, scale=0.05), 64)
+    down = ex.quantize_int4(normal(g, experts, hidden, inner, dtype=torch.bfloat16, scale=0.05), 128)
+    gate = normal(g, hidden, experts, dtype=torch.bfloat16, scale=0.1)
+
+    def step(x):
+        ids, w = ex.route(x @ gate, k)
+        order = ex.sort_by_expert(ids, experts)
+        h = ex.expert_matmul_int4(ex.dispatch(x, order), order.starts, order.counts, *up)
+        y = ex.expert_matmul_int4(h.relu(), order.starts, order.counts, *down)
+        return ex.combine(y, w, order), ids, w, h, y
+
+    x = normal(g, tokens, hidden, dtype=torch.bfloat16)
+    out, ids, w, h, y = step(x)
+    wu, wd = dequantized(*up, 64), dequantized(*down, 128)
+    for t in range(tokens):
+        total = torch.zeros(hidden, dtype=torch.float64, device="cuda")
+        for j in range(k):
+            e = ids[t, j]
+            mid = (wu[e] @ x[t].double()).to(torch.bfloat16).double().relu()
+            total += w[t, j].double() * (wd[e] @ mid).to(torch.bfloat16).double()
+        # the kernel and this loop round the middle and the expert's result to bf16 on sums that differ in fp32, so
+        # to neighbours at most (2 half steps each); the last rounding is one half step, fp32 errors less than one
+        mids = torch.stack([(wu[e].abs() @ x[t].double().abs()) for e in ids[t]])
+        size = sum(w[t, j].double() * (wd[ids[t, j]].abs() @ mids[j]) for j in range(k))
+        assert bool(((out[t].double() - total).abs() <= 6 * half_step(torch.bfloat16) * size).all())
+
+    stream = torch.cuda.Stream()
+    held = x.clone()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(held)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            captured = step(held)[0]
+        for seed in (1, 2):
+            fresh = normal(cuda(seed), tokens, hidden, dtype=torch.bfloat16)
+            stream.wait_stream(torch.cuda.current_stream())
+            held.copy_(fresh)
+            graph.replay()
+            assert torch.equal(captured, step(fresh)[0])
+    torch.cuda.current_stream().wait_stream(stream)
+
+
+@pytest.mark.gpu
+def test_autograd_is_refused_under_capture_and_plain_gradients_replay():
+    g = cuda(31)
+    x = normal(g, 16, 64).requires_grad_()
+    ids = torch.randint(0, 4, (16, 2), device="cuda", generator=g, dtype=torch.int32)
+    w = torch.rand(16, 2, device="cuda", generator=g)
+    order = ex.sort_by_expert(ids, 4)
+    eager = ex.dispatch(x, order)                      # an eager graph of the same leaf stays alive
+    grad = normal(g, 16, 64)
+    plain = x.detach()
+
+    def training_step():
+        rows = ex.dispatch(plain, order)
+        out = ex.combine(rows, w, order)
+        grad_rows, grad_w = ex.combine_backward(grad, rows, w, order)
+        return out, ex.dispatch_backward(grad_rows, order), grad_w
+
+    want = training_step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeFailure, match="capture"):
+            ex.dispatch(x, order)
+        got = training_step()
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    eager.sum().backward()
+    assert bool((x.grad == 2).all())
+
+
+@pytest.mark.gpu
+def test_out_over_an_input_is_refused():
+    cuda()
+    order = ex.sort_by_expert(torch.zeros(4, 1, dtype=torch.int32, device="cuda"), 1)
+    x = torch.zeros(6, 8, device="cuda")
+    with pytest.raises(RuntimeFailure, match="overlaps"):
+        ex.dispatch(x[:4], order, out=x[2:6])
+    with pytest.raises(RuntimeFailure, match="overlaps"):
+        ex.combine(x[:4], torch.zeros(4, 1, device="cuda"), order, out=x[:4])

@@ -133,7 +133,10 @@ def torch_flags():
 
 
 CUDA_SOURCES = ["cuda/interp.cu", "cuda/oneshot.cu", "cuda/helpers.cu", "cuda/probes.cu", "cuda/push.cu",
-                "cuda/fp8.cu", "runtime/symheap.cc", "runtime/cuda_ext.cc"]
+                "cuda/fp8.cu", "cuda/experts.cu", "cuda/int4.cu", "runtime/symheap.cc", "runtime/cuda_ext.cc",
+                "runtime/experts_ext.cc"]
+# built without --use_fast_math: subnormal values are kept, and exp and divisions are the accurate ones
+PRECISE_CUDA_SOURCES = frozenset({"experts.cu", "int4.cu"})
 
 
 @_serialized
@@ -161,7 +164,8 @@ def build_cuda_module(force: bool = False, jobs: int | None = None) -> Path:
     def compile_one(src: Path):
         obj = objdir / (src.name + ".o")
         if src.suffix == ".cu":
-            cmd = [str(CUDA_HOME / "bin" / "nvcc"), "-c", str(src), "-o", str(obj), *common, *nvflags]
+            flags = [f for f in nvflags if f != "--use_fast_math" or src.name not in PRECISE_CUDA_SOURCES]
+            cmd = [str(CUDA_HOME / "bin" / "nvcc"), "-c", str(src), "-o", str(obj), *common, *flags]
         else:
             cmd = ["g++", "-c", str(src), "-o", str(obj), *common, *ccflags]
         out = _run(cmd, "compile " + src.name)

@@ -1,0 +1,363 @@
+"""Mixture-of-experts operators on both sides of an AllToAll of tokens.
+
+* :func:`route` — the router's choice: the ``k`` largest logits of each token and their softmax weights.
+* :func:`sort_by_expert` — a stable sort of the (token, choice) assignments by expert, packed or with an equal
+  number of rows per expert (the equal parts an AllToAll exchanges).
+* :func:`dispatch` — every token copied to its rows; :func:`combine` — its rows weighted and summed back.
+* :func:`expert_matmul_int4` — the experts' matrix-vector products with 4-bit weights and group scales
+  (:func:`quantize_int4` lays weights out).
+
+All run on the current stream of their tensors' GPU, allocate nothing but their results, read nothing back to
+the host and can be captured into a CUDA graph.  ``route``, ``dispatch`` and ``combine`` take part in autograd;
+``route_backward``, ``dispatch_backward`` and ``combine_backward`` are the same gradients as plain calls, which is
+the form to capture: autograd refuses under capture, because the accumulation into a leaf that an eager graph
+still holds would run on a stream outside the capture.
+
+Matrices are ``[rows, hidden]`` with contiguous rows at any row stride (a column slice of a wider matrix, a row
+broadcast by ``expand``); ``out`` may be such a view too, must not overlap an input and is written whole.
+:class:`~vericcl_b200.models.ExpertExchange` puts these around an engine's AllToAll.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from vericcl_b200.errors import RuntimeFailure
+from vericcl_b200.ops import native
+
+MAX_EXPERTS = 1024
+MAX_CHOICES = 32
+INT4_GROUPS = (32, 64, 128)
+_DTYPES = frozenset({torch.float32, torch.bfloat16, torch.float16})
+_INT_MAX = 2 ** 31 - 1
+
+_module = None
+
+
+def _mod():
+    global _module
+    if _module is None:
+        _module = native.cuda()
+    return _module
+
+
+class ExpertOrder:
+    """Where each assignment's row is: the result of :func:`sort_by_expert`.
+
+    ``slot`` [tokens, k]: row of each assignment, -1 where it has none; ``source`` [rows]: assignment
+    (``token * k + choice``) of each row, -1 where a row has none; ``counts`` [experts]: rows in use;
+    ``starts`` [experts]: first row.  All int32 on the GPU.
+    """
+
+    __slots__ = ("slot", "source", "counts", "starts")
+
+    def __init__(self, slot, source, counts, starts):
+        self.slot, self.source, self.counts, self.starts = slot, source, counts, starts
+
+    @property
+    def rows(self) -> int:
+        return self.source.numel()
+
+
+# -- checks -----------------------------------------------------------------------------------------------
+
+def _matrix(t, name):
+    if t.dim() != 2 or t.dtype not in _DTYPES:
+        raise RuntimeFailure("%s must be a [rows, columns] matrix of float32, bfloat16 or float16" % name)
+    if t.size(1) > 1 and t.stride(1) != 1:
+        raise RuntimeFailure("%s must have contiguous rows (stride 1 in the last dimension)" % name)
+
+
+def _table(t, shape, dtype, name):
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise RuntimeFailure("%s must be a contiguous %s tensor of shape %s" % (name, dtype, list(shape)))
+
+
+def _order(order):
+    slot, source = order.slot, order.source
+    if slot.dtype != torch.int32 or slot.dim() != 2 or not slot.is_contiguous() or \
+            source.dtype != torch.int32 or source.dim() != 1 or not source.is_contiguous():
+        raise RuntimeFailure("an order holds contiguous int32 slot [tokens, k] and source [rows]")
+    return slot, source
+
+
+def _on_gpu(first, *others):
+    if not first.is_cuda:
+        raise RuntimeFailure("the expert operators need CUDA tensors")
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeFailure("the tensors are on different devices")
+
+
+def _result(out, rows, like, name, columns=None):
+    """Refuse an ``out`` that is not the result's shape and dtype or whose rows overlap each other or an input."""
+    if out is None:
+        return
+    columns = like.size(1) if columns is None else columns
+    if tuple(out.shape) != (rows, columns) or out.dtype != like.dtype:
+        raise RuntimeFailure("%s must be [%d, %d] of %s" % (name, rows, columns, like.dtype))
+    if (columns > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < columns):
+        raise RuntimeFailure("%s must have contiguous rows that do not overlap" % name)
+
+
+def _span(t):
+    lo = t.data_ptr()
+    return lo, lo + ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size() if t.numel() else lo
+
+
+def _apart(out, name, *inputs):
+    if out is None or not out.numel():
+        return
+    lo, hi = _span(out)
+    for t in inputs:
+        a, b = _span(t)
+        if a < hi and lo < b:
+            raise RuntimeFailure("%s overlaps an input" % name)
+
+
+def _learns(*tensors) -> bool:
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors):
+        return False
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeFailure("autograd under graph capture: capture the plain calls (detached inputs and the "
+                             "*_backward functions) instead")
+    return True
+
+
+def _no_out(out):
+    if out is not None:
+        raise RuntimeFailure("out= cannot be used with inputs that require gradients")
+
+
+def _rows_of(grad):
+    """A gradient from autograd as a matrix of contiguous rows (it may be expanded or transposed)."""
+    return grad if grad.size(1) <= 1 or grad.stride(1) == 1 else grad.contiguous()
+
+
+# -- router -----------------------------------------------------------------------------------------------
+
+def _check_route(logits, k):
+    _matrix(logits, "logits")
+    if not 1 <= logits.size(1) <= MAX_EXPERTS:
+        raise RuntimeFailure("logits must cover 1 to %d experts" % MAX_EXPERTS)
+    if not 1 <= k <= min(MAX_CHOICES, logits.size(1)):
+        raise RuntimeFailure("k must be 1 to min(%d, experts)" % MAX_CHOICES)
+    if logits.size(0) * logits.size(1) > 2 ** 40 or logits.size(0) * k > _INT_MAX:
+        raise RuntimeFailure("more than 2^31 - 1 assignments")
+
+
+def route(logits: torch.Tensor, k: int, *, renormalize: bool = True):
+    """``(ids, weights)``, int32 and float32 [tokens, k]: each token's ``k`` largest logits, the largest first
+    (ties to the lower expert), and their weights: the softmax over the chosen logits, or with
+    ``renormalize=False`` their share of the softmax over all.
+
+    A logit of -inf takes its expert out: a token with fewer than ``k`` experts left gets id -1 and weight 0 for
+    the rest.  A NaN logit is never chosen and makes the weights of its token NaN.
+    """
+    _check_route(logits, k)
+    _on_gpu(logits)
+    if _learns(logits):
+        return _Route.apply(logits, k, renormalize)
+    return _mod().route(logits, k, renormalize)
+
+
+def route_backward(logits, ids, weights, grad_weights, *, renormalize: bool = True) -> torch.Tensor:
+    """Gradient of ``route``'s weights with respect to ``logits`` [tokens, experts], in the logits' dtype."""
+    _check_route(logits, ids.size(-1) if ids.dim() else 0)
+    shape = (logits.size(0), ids.size(-1))
+    _table(ids, shape, torch.int32, "ids")
+    _table(weights, shape, torch.float32, "weights")
+    _table(grad_weights, shape, torch.float32, "grad_weights")
+    _on_gpu(logits, ids, weights, grad_weights)
+    return _mod().route_backward(logits, ids, weights, grad_weights, renormalize)
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, renormalize):
+        ids, weights = _mod().route(logits, k, renormalize)
+        ctx.renormalize = renormalize
+        ctx.save_for_backward(logits, ids, weights)
+        ctx.mark_non_differentiable(ids)
+        return ids, weights
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _, grad):
+        logits, ids, weights = ctx.saved_tensors
+        return _mod().route_backward(logits, ids, weights, grad.contiguous(), ctx.renormalize), None, None
+
+
+# -- sort, dispatch, combine ------------------------------------------------------------------------------
+
+def sort_by_expert(ids: torch.Tensor, experts: int, *, capacity: int | None = None) -> ExpertOrder:
+    """Rows for the assignments ``ids`` [tokens, k] (int32 or int64), grouped by expert and, within an expert, in
+    the order of the assignments.
+
+    Without ``capacity`` every assignment has a row: ``tokens * k`` rows, expert after expert without gaps.  With
+    it expert ``e`` owns the rows ``e * capacity ... (e + 1) * capacity - 1`` and assignments beyond them have
+    none.  An id outside ``[0, experts)`` (-1 for a padded token) has no row.
+    """
+    if ids.dim() != 2 or ids.dtype not in (torch.int32, torch.int64) or not ids.is_contiguous():
+        raise RuntimeFailure("ids must be a contiguous int32 or int64 tensor [tokens, k]")
+    if not 1 <= experts <= MAX_EXPERTS:
+        raise RuntimeFailure("1 to %d experts" % MAX_EXPERTS)
+    if capacity is not None and capacity < 1:
+        raise RuntimeFailure("a capacity is at least one row per expert")
+    if ids.size(1) < 1 or ids.size(1) > MAX_CHOICES:
+        raise RuntimeFailure("1 to %d choices per token" % MAX_CHOICES)
+    if ids.numel() > _INT_MAX or experts * (capacity or 0) > _INT_MAX:
+        raise RuntimeFailure("more than 2^31 - 1 assignments or rows")
+    _on_gpu(ids)
+    return ExpertOrder(*_mod().sort_by_expert(ids, experts, capacity or 0))
+
+
+def _check_dispatch(x, order, out, name):
+    slot, source = _order(order)
+    _matrix(x, name)
+    if x.size(0) != slot.size(0):
+        raise RuntimeFailure("%s has %d tokens, the order %d" % (name, x.size(0), slot.size(0)))
+    _result(out, source.numel(), x, "out")
+    _on_gpu(x, slot, source, out)
+    _apart(out, "out", x)
+    return slot, source
+
+
+def _check_combine(rows, weights, order, out, name):
+    slot, source = _order(order)
+    _matrix(rows, name)
+    if rows.size(0) != source.numel():
+        raise RuntimeFailure("%s has %d rows, the order %d" % (name, rows.size(0), source.numel()))
+    if weights is not None:
+        _table(weights, slot.shape, torch.float32, "weights")
+    _result(out, slot.size(0), rows, "out")
+    _on_gpu(rows, slot, source, weights, out)
+    _apart(out, "out", rows)
+    return slot, source
+
+
+def dispatch(x: torch.Tensor, order: ExpertOrder, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rows[r] = x[token of row r]`` [rows, hidden]; a row without an assignment is zero."""
+    slot, source = _check_dispatch(x, order, out, "x")
+    if _learns(x):
+        _no_out(out)
+        return _Dispatch.apply(x, slot, source)
+    return _mod().dispatch(x, slot, source, out)
+
+
+def dispatch_backward(grad_rows: torch.Tensor, order: ExpertOrder, *, out: torch.Tensor | None = None):
+    """Gradient of :func:`dispatch` with respect to ``x``: the sum of each token's rows, in fp32, rounded once."""
+    slot, source = _check_combine(grad_rows, None, order, out, "grad_rows")
+    return _mod().combine(grad_rows, None, slot, source, out)
+
+
+def combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder, *, out: torch.Tensor | None = None):
+    """``out[t] = sum over j of weights[t, j] * rows[slot[t, j]]`` [tokens, hidden], summed in fp32 in the order of
+    the choices and rounded once.  An assignment without a row adds nothing, whatever its weight; ``weights`` is
+    float32 [tokens, k]."""
+    slot, source = _check_combine(rows, weights, order, out, "rows")
+    if _learns(rows, weights):
+        _no_out(out)
+        return _Combine.apply(rows, weights, slot, source)
+    return _mod().combine(rows, weights, slot, source, out)
+
+
+def combine_backward(grad_out, rows, weights, order: ExpertOrder, *, out: torch.Tensor | None = None):
+    """``(grad_rows, grad_weights)`` of :func:`combine`: ``w * grad_out[t]`` at each assignment's row (zero in rows
+    without one; written to ``out`` where given) and the fp32 products ``<grad_out[t], rows[slot]>``, zero where an
+    assignment has no row."""
+    slot, source = _check_dispatch(grad_out, order, out, "grad_out")
+    _matrix(rows, "rows")
+    if tuple(rows.shape) != (source.numel(), grad_out.size(1)) or rows.dtype != grad_out.dtype:
+        raise RuntimeFailure("rows must be [%d, %d] of %s" % (source.numel(), grad_out.size(1), grad_out.dtype))
+    _table(weights, slot.shape, torch.float32, "weights")
+    _on_gpu(grad_out, rows, weights)
+    _apart(out, "out", rows)
+    return _mod().combine_backward(grad_out, rows, weights, slot, source, out)
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, slot, source):
+        ctx.save_for_backward(slot, source)
+        return _mod().dispatch(x, slot, source, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        slot, source = ctx.saved_tensors
+        return _mod().combine(_rows_of(grad), None, slot, source, None), None, None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, slot, source):
+        ctx.save_for_backward(rows, weights, slot, source)
+        return _mod().combine(rows, weights, slot, source, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        rows, weights, slot, source = ctx.saved_tensors
+        grad_rows, grad_weights = _mod().combine_backward(_rows_of(grad), rows, weights, slot, source, None)
+        return grad_rows, grad_weights, None, None
+
+
+# -- 4-bit products ---------------------------------------------------------------------------------------
+
+def quantize_int4(weight: torch.Tensor, group: int = 128, *, scale_dtype: torch.dtype | None = None):
+    """``(packed, scales)`` of a weight [..., n, inner]: uint8 [..., n, inner / 2] and [..., n, inner / group].
+
+    Value ``k`` of a row is ``(q - 8) * scale``: two 4-bit ``q`` a byte, the even ``k`` in the low half.  The scale of
+    a group, its largest magnitude / 7, is rounded to ``scale_dtype`` (the weight's by default) before the values
+    are, so its rounding moves the grid and adds no error of its own.  Done once when weights are loaded.
+    """
+    if weight.dim() < 2 or weight.dtype not in _DTYPES:
+        raise RuntimeFailure("a weight is [..., n, inner] of float32, bfloat16 or float16")
+    if group not in INT4_GROUPS or weight.size(-1) % group or not weight.size(-1):
+        raise RuntimeFailure("groups of 32, 64 or 128 that divide the inner size")
+    dtype = weight.dtype if scale_dtype is None else scale_dtype
+    if dtype not in _DTYPES:
+        raise RuntimeFailure("scales are float32, bfloat16 or float16")
+    w = weight.detach().float().unflatten(-1, (-1, group))
+    scales = (w.abs().amax(-1) / 7.0).to(dtype)
+    scales = torch.where(scales == 0, torch.ones_like(scales), scales)      # a group of zeros
+    q = (torch.round(w / scales.float()[..., None]).clamp_(-8, 7) + 8).to(torch.uint8).flatten(-2)
+    return (q[..., 0::2] | (q[..., 1::2] << 4)).contiguous(), scales.contiguous()
+
+
+def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, packed: torch.Tensor,
+                       scales: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[r] = W[e] @ rows[r]`` [rows, n] for the rows ``starts[s] ... starts[s] + counts[s] - 1`` of every
+    segment ``s``, whose expert is ``e = s % experts``; a row no segment covers is zero.
+
+    ``rows`` [rows, inner] is bfloat16 or float16; ``starts`` and ``counts`` int32 [segments] (an order's, or one
+    segment per source rank and expert after an AllToAll), a multiple of the experts, at most 1024, that ascend
+    and do not overlap; ``packed`` uint8 [experts, n, inner / 2] and ``scales`` [experts, n, inner / group] of the
+    rows' dtype or float32, as :func:`quantize_int4` gives them, in groups of 32, 64 or 128.  Products and sums are
+    fp32, rounded once.  No gradients: 4-bit weights are for serving.
+    """
+    _matrix(rows, "rows")
+    if rows.dtype == torch.float32:
+        raise RuntimeFailure("rows must be bfloat16 or float16")
+    if packed.dim() != 3 or packed.dtype != torch.uint8 or not packed.is_contiguous() or not packed.size(0) \
+            or packed.size(2) * 2 != rows.size(1):
+        raise RuntimeFailure("packed must be a contiguous uint8 tensor [experts, n, inner / 2]")
+    if scales.dim() != 3 or scales.shape[:2] != packed.shape[:2] or not scales.is_contiguous() or \
+            scales.dtype not in (torch.float32, rows.dtype):
+        raise RuntimeFailure("scales must be a contiguous tensor [experts, n, inner / group] of the rows' dtype or float32")
+    if not scales.size(2) or rows.size(1) % scales.size(2) or rows.size(1) // scales.size(2) not in INT4_GROUPS:
+        raise RuntimeFailure("groups of 32, 64 or 128 that divide the inner size")
+    segments = starts.numel()
+    if not 1 <= segments <= MAX_EXPERTS or segments % packed.size(0):
+        raise RuntimeFailure("1 to %d segments, a multiple of the experts" % MAX_EXPERTS)
+    _table(starts, (segments,), torch.int32, "starts")
+    _table(counts, (segments,), torch.int32, "counts")
+    if packed.data_ptr() % 16:
+        raise RuntimeFailure("packed must start on a 16-byte boundary")
+    if rows.requires_grad and torch.is_grad_enabled():
+        raise RuntimeFailure("4-bit products have no gradient: detach the rows")
+    _result(out, rows.size(0), rows, "out", packed.size(1))
+    _on_gpu(rows, starts, counts, packed, scales, out)
+    _apart(out, "out", rows)
+    return _mod().int4_product(rows, starts, counts, packed, scales, out)
