@@ -8,10 +8,13 @@
 // 8 rows of x as the other side; its sums are fp32.  One group's sum is scaled in fp32 and added to the total,
 // so a scale is never rounded into a weight.
 //
-// A lane holds weight rows g and g + 8 (g = lane / 4) and, of every group, the group / 4 values from
-// (lane % 4) * group / 4 on; x is staged in shared memory in that order, so a fragment is one conflict-free
-// 16-byte load.  A CTA of 8 warps covers 128 weight rows; a cluster of 1 to 8 CTAs splits the inner size and
-// joins its fp32 sums through distributed shared memory in the order of the CTAs.
+// A CTA of 8 warps covers 128 weight rows, 16 a warp.  Every warp streams its rows through its own ring of 2 KB
+// tiles (16 rows of 128 bytes, 256 inner values) that TMA fills, so no warp waits for another and the bytes in
+// flight cost no registers.  A lane holds, of two weight rows and of every group, the group / 4 values from
+// (lane % 4) * group / 4 on; x is staged in shared memory in that order, so its fragment is one conflict-free
+// 16-byte load.  A cluster of 1 to 8 CTAs splits the inner size and joins its fp32 sums through distributed
+// shared memory in the order of the CTAs.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -26,7 +29,18 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTileN = 128;           // weight rows of a CTA, 16 per warp
+constexpr int kItem = 32;             // rows of x of an item
+constexpr int kBoxK = 256;            // inner values of a TMA box: 128 bytes, the span of the swizzle
+constexpr int kBoxes = 2;             // boxes of a tile
+constexpr int kTileK = kBoxes * kBoxK;
+constexpr int kStages = 2;            // tiles in flight of a warp
+constexpr unsigned kBoxBytes = 16 * 128;
+constexpr int kStage = 16 * 1024;      // inner values x rows of x staged at a time: 32 KB
+constexpr unsigned kTileBytes = kBoxes * kBoxBytes;
 constexpr unsigned kFull = 0xffffffffu;
+
+// set when a copy did not arrive in time: the outputs it was for are NaN
+__device__ int late_copies = 0;
 
 __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
@@ -35,42 +49,78 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 
-__device__ __forceinline__ unsigned bits(__nv_bfloat162 v) { return *reinterpret_cast<unsigned*>(&v); }
-__device__ __forceinline__ unsigned bits(__half2 v) { return *reinterpret_cast<unsigned*>(&v); }
-
-// q - 8 of the 4-bit values at bits [0, 4) and [16, 20): 128 + q in bf16 and 1024 + q in fp16 have q in their
-// lowest mantissa bits, and the difference is exact
-template <typename T> __device__ __forceinline__ unsigned two_values(unsigned w);
-template <> __device__ __forceinline__ unsigned two_values<__nv_bfloat16>(unsigned w) {
-  const unsigned u = (w & 0x000f000fu) | 0x43004300u;
-  return bits(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), __float2bfloat162_rn(136.f)));
+// q - 8 of the 4-bit values at bits [0, 4) (HIGH 0) or [4, 8) (HIGH 1) of both halves of w, in two instructions.
+// fp16: 1024 + q (or 1024 + 16 q) has q in its mantissa, and one fma takes the 1024 off.  bf16 has too few mantissa
+// bits for the upper four, but below 2^-125 its numbers are evenly spaced, so the masked bits are already q 2^-133
+// or 16 q 2^-133; one fma makes them (q - 8) 2^-6, and the total is multiplied by 64 once at the end.  All exact.
+template <typename T, int HIGH>
+__device__ __forceinline__ unsigned two_values(unsigned w) {
+  constexpr unsigned mask = HIGH ? 0x00f000f0u : 0x000f000fu;
+  unsigned r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    r = w & mask;
+    asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(HIGH ? 0x7d007d00u : 0x7f007f00u), "r"(0xbe00be00u));
+  } else {
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(0x64006400u));   // (w & mask) | 1024
+    if (HIGH) asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x2c002c00u), "r"(0xd480d480u));
+    else asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64086408u));
+  }
+  return r;
 }
-template <> __device__ __forceinline__ unsigned two_values<__half>(unsigned w) {
-  const unsigned u = (w & 0x000f000fu) | 0x64006400u;
-  return bits(__hsub2(*reinterpret_cast<const __half2*>(&u), __float2half2_rn(1032.f)));
-}
+template <typename T> constexpr float kUnscale = std::is_same<T, __nv_bfloat16>::value ? 64.f : 1.f;
 
+// d = A B + (first ? 0 : d), the fragments i and i + 1
 template <typename T>
-__device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
-                                    unsigned b1) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma(float (&d)[4], const unsigned (&a)[4], const unsigned (&b)[4], int i, unsigned b0,
+                                    unsigned b1, bool first) {
+  const float c0 = first ? 0.f : d[0], c1 = first ? 0.f : d[1], c2 = first ? 0.f : d[2], c3 = first ? 0.f : d[3];
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[i]), "r"(b[i]), "r"(a[i + 1]), "r"(b[i + 1]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[i]), "r"(b[i]), "r"(a[i + 1]), "r"(b[i + 1]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// VEC words (8 values each) of one lane's part of a group, read once
+// VEC words (8 values each) of one lane's part of a group
 template <int VEC>
-__device__ __forceinline__ void load_words(unsigned (&w)[VEC], const unsigned char* p) {
-  if constexpr (VEC == 4)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "l"(p));
-  else if constexpr (VEC == 2)
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-  else
-    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+__device__ __forceinline__ void load_words(unsigned (&w)[VEC], const unsigned char* at) {
+  if constexpr (VEC == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(at);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (VEC == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(at);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const unsigned*>(at);
+  }
+}
+
+__device__ __forceinline__ void barrier_init(unsigned bar) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar) : "memory");
+}
+
+// one tile of 16 weight rows x 256 bytes into shared memory; the barrier counts its bytes (what lies past the end
+// of a row arrives as zeros and counts too)
+__device__ __forceinline__ void load_tile(const CUtensorMap* map, unsigned to, unsigned bar, int x, int y) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kTileBytes) : "memory");
+#pragma unroll
+  for (int i = 0; i < kBoxes; ++i)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(to + i * kBoxBytes), "l"(map), "r"(x + i * (kBoxK / 2)), "r"(y), "r"(bar) : "memory");
+}
+
+// Waits until the barrier's phase is over; false after about a second without it.
+__device__ __forceinline__ bool wait_tile(unsigned bar, unsigned phase) {
+  for (int i = 0; i < (1 << 20); ++i) {
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(phase), "r"(1000u) : "memory");
+    if (done) return true;
+  }
+  return false;
 }
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -94,42 +144,220 @@ __device__ __forceinline__ float remote_f(unsigned addr, unsigned rank) {
   return v;
 }
 
+// PAIR groups of 16 weight rows times COLS x 8 rows of x, scaled and added to acc.  `x` is the lane's first unit.
+// The groups' products alternate, and with one column each group's sum is kept in two halves, so that a product
+// seldom waits for the one before it.  A lane whose row of x does not exist computes with what lies there: columns
+// of a product do not mix, and that column is not written.
+template <typename T, typename S, int VEC, int COLS, int PAIR>
+__device__ __forceinline__ void group_product(float (&acc)[COLS][4], const unsigned char* tile, unsigned at, int u0,
+                                              const uint4* x, const S* scale) {
+  constexpr int HALVES = COLS == 1 ? 2 : 1;
+  unsigned ra[PAIR][VEC], rb[PAIR][VEC];
+  float part[PAIR][HALVES][COLS][4];
+#pragma unroll
+  for (int p = 0; p < PAIR; ++p) {
+    // within a box the groups differ in the chunk bits, which the swizzle leaves to an exclusive or
+    const int u = u0 + p, in_box = kBoxK / (32 * VEC);
+    const unsigned char* from = tile + (at ^ (16 * VEC * (u % in_box))) + u / in_box * kBoxBytes;
+    load_words<VEC>(ra[p], from);
+    load_words<VEC>(rb[p], from + 1024);
+  }
+#pragma unroll
+  for (int v = 0; v < VEC; ++v)
+#pragma unroll
+    for (int p = 0; p < PAIR; ++p) {
+      const unsigned wa = ra[p][v], wb = rb[p][v];
+      const unsigned va[4] = {two_values<T, 0>(wa), two_values<T, 1>(wa), two_values<T, 0>(wa >> 8), two_values<T, 1>(wa >> 8)};
+      const unsigned vb[4] = {two_values<T, 0>(wb), two_values<T, 1>(wb), two_values<T, 0>(wb >> 8), two_values<T, 1>(wb >> 8)};
+#pragma unroll
+      for (int t = 0; t < COLS; ++t) {
+        const uint4 b = x[((p * VEC + v) * COLS + t) * 32];
+        mma<T>(part[p][0][t], va, vb, 0, b.x, b.y, v == 0);
+        mma<T>(part[p][HALVES - 1][t], va, vb, 2, b.z, b.w, HALVES == 2 && v == 0);
+      }
+    }
+#pragma unroll
+  for (int p = 0; p < PAIR; ++p) {
+    const float sa = to_f(scale[p * kTileN]), sb = to_f(scale[p * kTileN + 8]);
+#pragma unroll
+    for (int t = 0; t < COLS; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float sum = part[p][0][t][i];
+        if constexpr (HALVES == 2) sum += part[p][1][t][i];
+        acc[t][i] = fmaf(i < 2 ? sa : sb, sum, acc[t][i]);
+      }
+  }
+}
+
 struct Geometry {
-  long long slice;     // inner values of one CTA of the cluster, a multiple of the chunk's group
-  int chunk;           // inner values staged at a time
+  long long slice;     // inner values of one CTA of the cluster, whole tiles
   int aligned;         // rows of x can be read 16 bytes at a time
   unsigned n_tiles, items;
 };
 
-// rows [first, first + count) of segment s inside the matrix
-__device__ __forceinline__ void segment(const Int4Args& a, int s, long long& first, long long& count) {
-  const long long lo = a.starts[s], hi = lo + a.counts[s];
-  first = lo < 0 ? 0 : lo;
-  count = (hi > a.rows ? a.rows : hi) - first;
-  if (count < 0) count = 0;
+struct Item {
+  int expert, row0, rows;    // rows of x: row0 ... row0 + rows - 1, at most 32
+  long long n0;              // the CTA's first weight row
+  int k_lo, k_hi;            // its inner values
+};
+
+// One CTA's part of an item of at most 8 * COLS rows of x: its sums over its inner values, [row of x][weight row],
+// left in shared memory.
+template <typename T, typename S, int VEC, int COLS>
+__device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args& a, const Geometry& geo, const Item& it,
+                                          unsigned char* smem, unsigned bars) {
+  constexpr int GROUP = 32 * VEC, UNITS = kTileK / GROUP;               // groups of a tile
+  constexpr int CHUNK = kStage / (8 * COLS) / kTileK * UNITS;           // groups of a stage, whole tiles
+  constexpr int PAIR = COLS <= 2 ? 2 : 1;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
+  const int groups = (int)(a.inner / GROUP), units = (it.k_hi - it.k_lo) / GROUP, tiles = (units + UNITS - 1) / UNITS;
+  const long long base = (long long)it.expert * a.n;
+  // the warp's ring; a warp whose rows are all past the last has nothing to do
+  const unsigned char* ring = smem + warp * (kStages * kTileBytes);
+  const unsigned to = (unsigned)__cvta_generic_to_shared(ring), bar = bars + warp * (kStages * 8);
+  const bool busy = it.n0 + warp * 16 < a.n;
+  const int y = (int)(base + it.n0) + warp * 16;
+  if (busy && lane == 0)
+    for (int i = 0; i < kStages && i < tiles; ++i)
+      load_tile(map, to + i * kTileBytes, bar + 8 * i, it.k_lo / 2 + i * (kTileK / 2), y);
+  // rows are dealt to the lanes so that the lanes of one shared-memory phase meet different banks of the
+  // 128-byte swizzle (16-byte chunk c of row r is at c ^ (r % 8))
+  const int row = VEC == 4 ? (g & 1) * 4 + (g >> 1) : VEC == 2 ? (g & 3) * 2 + (g >> 2) : g;
+  const unsigned lane_at = row * 128 + (((tq * VEC / 4) ^ row) << 4) + (tq * VEC % 4) * 4;
+  const T* x = static_cast<const T*>(a.x) + it.row0 * a.x_stride + it.k_lo;
+  const S* scales = static_cast<const S*>(a.scales) + (base + min(it.n0 + (tid & (kTileN - 1)), a.n - 1)) * groups + it.k_lo / GROUP;
+  unsigned char* staged = smem + (kThreads / 32) * kStages * kTileBytes;
+  uint4* xs = reinterpret_cast<uint4*>(staged);                         // [groups * VEC][8 * COLS][4]
+  S* sc = reinterpret_cast<S*>(staged + kStage * 2);                    // [groups][kTileN]
+  float acc[COLS][4];
+#pragma unroll
+  for (int t = 0; t < COLS; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+  int slot = 0;
+  unsigned phase = 0;
+  int late = -1;                            // the tile that did not come
+
+  for (int c0 = 0; c0 < units; c0 += CHUNK) {
+    const int here = min(CHUNK, units - c0), eighths = here * (GROUP / 8);
+    if (c0) __syncthreads();                // the stage before has been read
+    // x as 16-byte units of 8 inner values in the order 0 4 1 5 2 6 3 7; four loads are in flight per thread
+    {
+      const T* p = x + (long long)c0 * GROUP;
+      int token = tid / eighths, k8 = tid - token * eighths;
+      while (token < it.rows) {
+        uint4 v[4];
+        int at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          at[i] = -1;
+          if (token < it.rows) {
+            const T* from = p + token * a.x_stride + 8 * k8;
+            if (geo.aligned) {
+              v[i] = *reinterpret_cast<const uint4*>(from);
+            } else {
+              __align__(16) T e[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) e[j] = from[j];
+              v[i] = *reinterpret_cast<uint4*>(e);
+            }
+            const int grp = k8 / (4 * VEC), in = k8 % (4 * VEC);        // in = (lane % 4) * VEC + word
+            at[i] = ((grp * VEC + in % VEC) * (8 * COLS) + token) * 4 + in / VEC;
+          }
+          k8 += kThreads;
+          while (k8 >= eighths) { k8 -= eighths; ++token; }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (at[i] >= 0)
+            xs[at[i]] = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
+                                   __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
+      }
+    }
+    for (int u0 = tid / kTileN; u0 < here; u0 += 8 * (kThreads / kTileN)) {
+      S v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (u0 + i * (kThreads / kTileN) < here) v[i] = scales[c0 + u0 + i * (kThreads / kTileN)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (u0 + i * (kThreads / kTileN) < here) sc[(u0 + i * (kThreads / kTileN)) * kTileN + (tid & (kTileN - 1))] = v[i];
+    }
+    __syncthreads();
+    const uint4* xw = xs + g * 4 + tq;
+    const S* sw = sc + warp * 16 + row;
+    if (busy)
+      for (int u0 = 0; u0 < here; u0 += UNITS) {
+        if (late < 0 && !__all_sync(kFull, wait_tile(bar + 8 * slot, phase))) late = (c0 + u0) / UNITS;
+        const unsigned char* tile = ring + slot * kTileBytes;
+        if (u0 + UNITS <= here) {
+#pragma unroll
+          for (int u = 0; u < UNITS; u += PAIR)
+            group_product<T, S, VEC, COLS, PAIR>(acc, tile, lane_at, u, xw + u * VEC * COLS * 32, sw + u * kTileN);
+        } else {
+          for (int u = 0; u0 + u < here; ++u)
+            group_product<T, S, VEC, COLS, 1>(acc, tile, lane_at, u, xw + u * VEC * COLS * 32, sw + u * kTileN);
+        }
+        xw += UNITS * VEC * COLS * 32;
+        sw += UNITS * kTileN;
+        __syncwarp();                       // the tile has been read by every lane
+        const int coming = (c0 + u0) / UNITS + kStages;
+        if (lane == 0 && coming < tiles && late < 0)
+          load_tile(map, to + slot * kTileBytes, bar + 8 * slot, it.k_lo / 2 + coming * (kTileK / 2), y);
+        if (++slot == kStages) { slot = 0; phase ^= 1; }
+      }
+  }
+  float unscale = kUnscale<T>;
+  if (late >= 0) {                          // a last chance for what is in flight, then NaN
+    if (lane == 0) atomicExch(&late_copies, 1);
+    for (int i = late; i < tiles && i < late + kStages; ++i) wait_tile(bar + 8 * (i % kStages), i / kStages & 1);
+    unscale = __int_as_float(0x7fffffff);
+  }
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(staged);
+#pragma unroll
+  for (int t = 0; t < COLS; ++t) {
+    float* at = sums + (8 * t + 2 * tq) * kTileN + warp * 16 + row;
+    at[0] = acc[t][0] * unscale;
+    at[kTileN] = acc[t][1] * unscale;
+    at[8] = acc[t][2] * unscale;
+    at[kTileN + 8] = acc[t][3] * unscale;
+  }
 }
 
-template <typename T, typename S, int VEC, int NT>
-__global__ void __launch_bounds__(kThreads) int4_product_kernel(Int4Args a, Geometry geo) {
-  constexpr int GROUP = 32 * VEC;
-  constexpr int TOK = 8 * NT;               // rows of x of one item
-  constexpr int DEPTH = 16 / VEC;           // groups in flight per warp: 4 KB
-  extern __shared__ __align__(16) unsigned char smem[];
+template <typename T, typename S, int VEC>
+__global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_constant__ CUtensorMap map, Int4Args a,
+                                                                Geometry geo) {
+  extern __shared__ unsigned char dynamic[];
+  // the swizzle's pattern repeats every 1024 bytes of the address
+  unsigned char* smem = dynamic + (-(unsigned)__cvta_generic_to_shared(dynamic) & 1023u);
+  __shared__ __align__(8) unsigned long long bars[kThreads / 32][kStages];
   __shared__ int pick[3];                   // segment, first row, rows of this CTA's item
-  __shared__ int scan[kThreads / 32];
+  __shared__ int2 scan[kThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned rank = cluster_rank(), ranks = cluster_size();
   const int item = (int)(blockIdx.x / ranks / geo.n_tiles);
   const long long n0 = (long long)(blockIdx.x / ranks % geo.n_tiles) * kTileN;
 
-  // which segment and rows: the items count the segments' tiles of TOK rows
+  // which segment and rows: the items count the segments' tiles of kItem rows
+  int covered = 0;                          // rows that some segment covers
   {
-    const int per = (a.segments + kThreads - 1) / kThreads, s0 = tid * per;
-    int mine = 0;
-    for (int s = s0; s < s0 + per && s < a.segments; ++s) {
-      long long first, count;
-      segment(a, s, first, count);
-      mine += (int)((count + TOK - 1) / TOK);
+    constexpr int PER = 1024 / kThreads;    // at most 1024 segments, PER consecutive ones a thread
+    int first[PER], count[PER], mine = 0, rows = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int s = tid * PER + i;
+      first[i] = s < a.segments ? a.starts[s] : 0;
+      count[i] = s < a.segments ? a.counts[s] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {         // kept inside the matrix
+      const long long lo = first[i], hi = min(lo + count[i], a.rows);
+      first[i] = max(first[i], 0);
+      count[i] = (int)max(hi - first[i], 0ll);
+      mine += (count[i] + kItem - 1) / kItem;
+      rows += count[i];
     }
     int x = mine;
 #pragma unroll
@@ -137,183 +365,102 @@ __global__ void __launch_bounds__(kThreads) int4_product_kernel(Int4Args a, Geom
       const int y = __shfl_up_sync(kFull, x, off);
       if (lane >= off) x += y;
     }
-    if (lane == 31) scan[warp] = x;
+    rows = __reduce_add_sync(kFull, rows);
+    if (lane == 31) scan[warp] = make_int2(x, rows);
     if (tid == 0) pick[0] = -1;
+    if (tid < kThreads / 32 * kStages) barrier_init((unsigned)__cvta_generic_to_shared(&bars[0][0] + tid));
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
     int before = x - mine;
-    for (int w = 0; w < warp; ++w) before += scan[w];
-    if (item >= before && item < before + mine)
-      for (int s = s0; s < s0 + per && s < a.segments; ++s) {
-        long long first, count;
-        segment(a, s, first, count);
-        const int tiles = (int)((count + TOK - 1) / TOK);
-        if (item >= before && item < before + tiles) {
-          const long long at = (long long)(item - before) * TOK;
-          pick[0] = s;
-          pick[1] = (int)(first + at);
-          pick[2] = (int)(count - at < TOK ? count - at : TOK);
-        }
-        before += tiles;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const int2 got = scan[w];
+      if (w < warp) before += got.x;
+      covered += got.y;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int tiles = (count[i] + kItem - 1) / kItem, at = (item - before) * kItem;
+      if (item >= before && item < before + tiles) {
+        pick[0] = tid * PER + i;
+        pick[1] = first[i] + at;
+        pick[2] = min(count[i] - at, kItem);
       }
+      before += tiles;
+    }
     __syncthreads();
   }
 
   if (pick[0] >= 0) {                       // the same for every CTA of the cluster
-    const int expert = pick[0] % a.experts, row0 = pick[1], tokens = pick[2];
-    const int g = lane >> 2, tq = lane & 3;
-    const long long groups = a.inner / GROUP;
-    const long long k_lo = rank * geo.slice, k_hi = min(a.inner, k_lo + geo.slice);
-    const long long n_a = n0 + warp * 16 + g, n_b = n_a + 8;
-    const long long base = (long long)expert * a.n;
-    // rows past the last are clamped to it and not written
-    const unsigned char* qa = a.packed + (base + min(n_a, a.n - 1)) * (a.inner / 2) + tq * (4 * VEC);
-    const unsigned char* qb = a.packed + (base + min(n_b, a.n - 1)) * (a.inner / 2) + tq * (4 * VEC);
-    const T* x = static_cast<const T*>(a.x);
-    uint4* xs = reinterpret_cast<uint4*>(smem);                       // [chunk / 32 units][TOK][4]
-    S* sc = reinterpret_cast<S*>(smem + (size_t)geo.chunk * TOK * 2); // [chunk / GROUP][kTileN]
-    float acc[NT][4];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-
-    for (long long c0 = k_lo; c0 < k_hi; c0 += geo.chunk) {
-      const int len = (int)min((long long)geo.chunk, k_hi - c0);      // a multiple of GROUP
-      const int units = len / GROUP;
-      const unsigned char* wa = qa + c0 / 2;
-      const unsigned char* wb = qb + c0 / 2;
-      unsigned ra[DEPTH][VEC], rb[DEPTH][VEC];
-#pragma unroll
-      for (int d = 0; d < DEPTH; ++d)
-        if (d < units) {
-          load_words<VEC>(ra[d], wa + d * (GROUP / 2));
-          load_words<VEC>(rb[d], wb + d * (GROUP / 2));
-        }
-      // stage x: 16-byte units of 8 inner values in the order 0 4 1 5 2 6 3 7
-      for (int i = tid; i < len / 8 * TOK; i += kThreads) {
-        const int token = i / (len / 8), k8 = i % (len / 8);
-        T v[8];
-        if (token < tokens) {
-          const T* p = x + (row0 + token) * a.x_stride + c0 + 8 * k8;
-          if (geo.aligned) {
-            *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = p[e];
-          }
-        } else {
-          *reinterpret_cast<uint4*>(v) = make_uint4(0, 0, 0, 0);
-        }
-        T o[8] = {v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};
-        const int grp = k8 / (4 * VEC), in = k8 % (4 * VEC);          // in = tq * VEC + word
-        xs[((grp * VEC + in % VEC) * TOK + token) * 4 + in / VEC] = *reinterpret_cast<uint4*>(o);
-      }
-      for (int i = tid; i < units * kTileN; i += kThreads) {
-        const int row = i / units, u = i % units;
-        const long long n = min(n0 + row, a.n - 1);
-        sc[u * kTileN + row] = static_cast<const S*>(a.scales)[(base + n) * groups + c0 / GROUP + u];
-      }
-      __syncthreads();
-      for (int u0 = 0; u0 < units; u0 += DEPTH) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-          const int u = u0 + d;
-          if (u < units) {
-            float part[NT][4];
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) part[t][i] = 0.f;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-              unsigned va[4], vb[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                va[i] = two_values<T>(ra[d][v] >> (4 * i));
-                vb[i] = two_values<T>(rb[d][v] >> (4 * i));
-              }
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-                if (8 * t < tokens) {
-                  const uint4 b = xs[((u * VEC + v) * TOK + 8 * t + g) * 4 + tq];
-                  mma<T>(part[t], va[0], vb[0], va[1], vb[1], b.x, b.y);
-                  mma<T>(part[t], va[2], vb[2], va[3], vb[3], b.z, b.w);
-                }
-            }
-            if (u + DEPTH < units) {
-              load_words<VEC>(ra[d], wa + (u + DEPTH) * (GROUP / 2));
-              load_words<VEC>(rb[d], wb + (u + DEPTH) * (GROUP / 2));
-            }
-            const float sa = to_f(sc[u * kTileN + warp * 16 + g]), sb = to_f(sc[u * kTileN + warp * 16 + g + 8]);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              acc[t][0] = fmaf(sa, part[t][0], acc[t][0]);
-              acc[t][1] = fmaf(sa, part[t][1], acc[t][1]);
-              acc[t][2] = fmaf(sb, part[t][2], acc[t][2]);
-              acc[t][3] = fmaf(sb, part[t][3], acc[t][3]);
-            }
-          }
-        }
-      }
-      __syncthreads();
+    Item it;
+    it.expert = pick[0] % a.experts;
+    it.row0 = pick[1];
+    it.rows = pick[2];
+    it.n0 = n0;
+    it.k_lo = (int)min(a.inner, rank * geo.slice);
+    it.k_hi = (int)min(a.inner, it.k_lo + geo.slice);
+    const unsigned bar = (unsigned)__cvta_generic_to_shared(&bars[0][0]);
+    switch ((it.rows + 7) / 8) {
+      case 1: item_sums<T, S, VEC, 1>(&map, a, geo, it, smem, bar); break;
+      case 2: item_sums<T, S, VEC, 2>(&map, a, geo, it, smem, bar); break;
+      case 3: item_sums<T, S, VEC, 3>(&map, a, geo, it, smem, bar); break;
+      default: item_sums<T, S, VEC, 4>(&map, a, geo, it, smem, bar); break;
     }
-
-    // join the cluster's sums: sums[token][row], CTA `rank` finishes every ranks-th part of the outputs
-    float* sums = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int token = 8 * t + 2 * tq, row = warp * 16 + g;
-      sums[token * kTileN + row] = acc[t][0];
-      sums[(token + 1) * kTileN + row] = acc[t][1];
-      sums[token * kTileN + row + 8] = acc[t][2];
-      sums[(token + 1) * kTileN + row + 8] = acc[t][3];
-    }
+    // join the cluster's sums: CTA `rank` finishes every ranks-th part of the outputs
+    float* sums = reinterpret_cast<float*>(smem + (kThreads / 32) * kStages * kTileBytes);
     if (ranks > 1) cluster_sync(); else __syncthreads();
     const unsigned sums_at = (unsigned)__cvta_generic_to_shared(sums);
     T* out = static_cast<T*>(a.out);
-    for (int i = rank * kThreads + tid; i < tokens * kTileN; i += ranks * kThreads) {
-      const int token = i / kTileN, row = i % kTileN;
+    for (int i = rank * kThreads + tid; i < it.rows * kTileN; i += ranks * kThreads) {
+      const int token = i / kTileN, n = i % kTileN;
       float v = 0.f;
       for (unsigned r = 0; r < ranks; ++r) v += remote_f(sums_at + 4u * i, r);
-      if (n0 + row < a.n) out[(row0 + token) * a.out_stride + n0 + row] = from_f<T>(v);
+      if (n0 + n < a.n) out[(it.row0 + token) * a.out_stride + n0 + n] = from_f<T>(v);
     }
     if (ranks > 1) cluster_sync();          // the sums stay until every CTA has read them
   }
 
   // rows that no segment covers are zero; row r belongs to item r mod the items
-  if (rank == 0)
+  if (rank == 0 && covered < a.rows)
     for (long long r = item + (long long)warp * geo.items; r < a.rows; r += 8ll * geo.items) {
-      bool covered = false;
+      bool inside = false;
       for (int s = lane; s < a.segments; s += 32) {
         const long long lo = a.starts[s];
-        covered |= r >= lo && r < lo + a.counts[s];
+        inside |= r >= lo && r < lo + a.counts[s];
       }
-      if (!__any_sync(kFull, covered))
+      if (!__any_sync(kFull, inside))
         for (int c = lane; c < kTileN && n0 + c < a.n; c += 32) static_cast<T*>(a.out)[r * a.out_stride + n0 + c] = from_f<T>(0.f);
     }
 }
 
-template <typename T, typename S, int VEC, int NT>
+template <typename T, typename S, int VEC>
 cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
-  constexpr int TOK = 8 * NT, GROUP = 32 * VEC;
-  // tiles: every segment's last may be partial
-  const long long items = (a.rows + TOK - 1) / TOK + (a.segments < a.rows ? a.segments : a.rows) - 1;
+  constexpr int GROUP = 32 * VEC;
+  // items: every segment's last may be partial
+  const long long items = (a.rows + kItem - 1) / kItem + (a.segments < a.rows ? a.segments : a.rows) - 1;
   const long long n_tiles = (a.n + kTileN - 1) / kTileN;
-  // split the inner size until the GPU is full, as long as a CTA keeps 256 values
+  // split the inner size until the GPU is full, as long as a CTA keeps a tile
   int ranks = 1;
-  while (ranks < 8 && n_tiles * items * ranks < 148 * 4 && a.inner / (2 * ranks) >= 256) ranks *= 2;
+  while (ranks < 8 && n_tiles * items * ranks * 2 <= 148 * 2 && a.inner / (2 * ranks) >= kTileK) ranks *= 2;
   Geometry geo{};
-  const long long groups = a.inner / GROUP;
-  geo.slice = (groups + ranks - 1) / ranks * GROUP;
-  const long long most = 2048 / NT;
-  geo.chunk = (int)(geo.slice < most ? geo.slice : most);
+  const long long tiles = (a.inner + kTileK - 1) / kTileK;
+  geo.slice = (tiles + ranks - 1) / ranks * kTileK;
   geo.n_tiles = (unsigned)n_tiles;
   geo.items = (unsigned)items;
   geo.aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 8 == 0;
-  size_t bytes = (size_t)geo.chunk * TOK * 2 + (size_t)geo.chunk / GROUP * kTileN * sizeof(S);
-  const size_t sums = sizeof(float) * TOK * kTileN;
+  size_t bytes = (size_t)kStage * 2 + (size_t)kStage / 8 / GROUP * kTileN * sizeof(S);
+  const size_t sums = sizeof(float) * kItem * kTileN;
   if (bytes < sums) bytes = sums;
-  auto kernel = int4_product_kernel<T, S, VEC, NT>;
+  bytes += kThreads / 32 * kStages * kTileBytes + 1024;
+  CUtensorMap map;
+  const cuuint64_t size[2] = {(cuuint64_t)(a.inner / 2), (cuuint64_t)a.experts * a.n}, pitch[1] = {(cuuint64_t)(a.inner / 2)};
+  const cuuint32_t box[2] = {128, 16}, step[2] = {1, 1};
+  if (cuTensorMapEncodeTiled(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<unsigned char*>(a.packed), size, pitch, box,
+                             step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cudaErrorInvalidValue;
+  auto kernel = int4_product_kernel<T, S, VEC>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t config{};
@@ -329,22 +476,19 @@ cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
   attr.val.clusterDim.z = 1;
   config.attrs = &attr;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, a, geo);
-}
-
-template <typename T, typename S, int VEC>
-cudaError_t launch_tokens(const Int4Args& a, cudaStream_t stream) {
-  return a.rows <= 8 ? launch<T, S, VEC, 1>(a, stream) : launch<T, S, VEC, 4>(a, stream);
+  return cudaLaunchKernelEx(&config, kernel, map, a, geo);
 }
 
 template <typename T, typename S>
 cudaError_t launch_group(const Int4Args& a, cudaStream_t stream) {
-  if (a.group == 128) return launch_tokens<T, S, 4>(a, stream);
-  if (a.group == 64) return launch_tokens<T, S, 2>(a, stream);
-  return launch_tokens<T, S, 1>(a, stream);
+  if (a.group == 128) return launch<T, S, 4>(a, stream);
+  if (a.group == 64) return launch<T, S, 2>(a, stream);
+  return launch<T, S, 1>(a, stream);
 }
 
 }  // namespace
+
+cudaError_t int4_late_copies(int* count) { return cudaMemcpyFromSymbol(count, late_copies, sizeof(int)); }
 
 cudaError_t launch_int4_product(const Int4Args& a, cudaStream_t stream) {
   if (a.rows == 0 || a.n == 0) return cudaSuccess;

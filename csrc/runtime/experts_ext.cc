@@ -217,7 +217,8 @@ Tensor int4_product(const Tensor& x, const Tensor& starts, const Tensor& counts,
               segments % packed.size(0) == 0 && segments <= kMaxExperts, "segments are a multiple of the experts");
   TORCH_CHECK(x.scalar_type() != at::kFloat && (scales.scalar_type() == at::kFloat || scales.scalar_type() == x.scalar_type()),
               "16-bit rows, scales of their type or fp32");
-  TORCH_CHECK(x.size(0) <= INT_MAX && packed.size(1) <= INT_MAX, "more than 2^31 - 1 rows or outputs");
+  TORCH_CHECK(x.size(0) <= INT_MAX && packed.size(0) * packed.size(1) <= INT_MAX && x.size(1) <= INT_MAX,
+              "more than 2^31 - 1 rows, weight rows or inner values");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 == 0, "packed starts on a 16-byte boundary");
   c10::cuda::CUDAGuard guard(x.device());
   Tensor y;
@@ -262,4 +263,9 @@ void bind_experts(py::module_& m) {
   m.def("combine", &combine);
   m.def("combine_backward", &combine_backward);
   m.def("int4_product", &int4_product);
+  m.def("int4_late_copies", []() {
+    int flag = 0;
+    done(int4_late_copies(&flag), "read the late-copy flag");
+    return flag != 0;
+  });
 }

@@ -353,6 +353,8 @@ def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.T
         raise RuntimeFailure("1 to %d segments, a multiple of the experts" % MAX_EXPERTS)
     _table(starts, (segments,), torch.int32, "starts")
     _table(counts, (segments,), torch.int32, "counts")
+    if rows.size(0) > _INT_MAX or packed.size(0) * packed.size(1) > _INT_MAX or rows.size(1) > _INT_MAX:
+        raise RuntimeFailure("more than 2^31 - 1 rows, weight rows or inner values")
     if packed.data_ptr() % 16:
         raise RuntimeFailure("packed must start on a 16-byte boundary")
     if rows.requires_grad and torch.is_grad_enabled():
