@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cstdint>
+
 #include "vb/launch.h"
 
 namespace vb {
@@ -178,12 +180,34 @@ cudaError_t route_any(const RouteArgs& a, cudaStream_t stream) {
 
 // ---- stable sort by expert ------------------------------------------------------------------------------
 //
-// Each warp owns a contiguous run of assignments.  Pass 1 counts each warp's assignments per expert (the lanes
-// that hold one expert elect a leader with match_any, so no count depends on the order of atomics), a scan over
-// the warps and the experts turns the counts into each warp's first place per expert, pass 2 hands the places
-// out in the order of the assignments.
-constexpr int kSortThreads = 1024;
-constexpr int kSortWarps = kSortThreads / 32;
+// One cluster of 1 to 16 CTAs; every warp owns a contiguous run of assignments.  Pass 1 counts each warp's
+// assignments per expert (the lanes that hold one expert elect a leader with match_any, so no count depends on the
+// order of atomics), scans over the warps, over the CTAs (through distributed shared memory) and over the experts
+// turn the counts into each warp's first place per expert, pass 2 hands the places out in the order of the
+// assignments.  One launch and no workspace: what it costs is the latency of these steps, not its few bytes.
+constexpr int kSortWarps = 32;         // most warps of a CTA
+constexpr int kSortCtas = 16;          // most CTAs of the cluster
+constexpr int kSortRun = 128;          // assignments of a warp before another warp or CTA is added
+
+__device__ __forceinline__ unsigned cluster_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned cluster_size() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ int remote_int(const int* p, unsigned rank) {
+  unsigned there;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
+  return v;
+}
 
 template <typename I>
 __device__ __forceinline__ int expert_of(const SortArgs& a, long long i, long long hi) {
@@ -192,157 +216,305 @@ __device__ __forceinline__ int expert_of(const SortArgs& a, long long i, long lo
   return e >= 0 && e < a.experts ? (int)e : -1;
 }
 
+__device__ __forceinline__ int inclusive_scan(int x, int lane) {
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int y = __shfl_up_sync(kFull, x, off);
+    if (lane >= off) x += y;
+  }
+  return x;
+}
+
 template <typename I>
-__global__ void __launch_bounds__(kSortThreads) sort_kernel(SortArgs a) {
+__global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
   extern __shared__ int sm[];
+  constexpr int AHEAD = 4;              // loads of a lane in flight
   const int E = a.experts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int* hist = sm;                       // [kSortWarps][E]
-  int* first = sm + kSortWarps * E;     // [E] first row of each expert
-  int* total = first + E;               // [E]
-  for (int i = tid; i < kSortWarps * E; i += kSortThreads) hist[i] = 0;
+  const int threads = blockDim.x, warps = threads >> 5, pitch = E | 1;   // an odd pitch: a column meets all banks
+  const int rank = (int)cluster_rank(), ctas = (int)cluster_size();
+  int* hist = sm;                       // [warps][pitch] counts, then first places
+  int* total = sm + warps * pitch;      // [E] of this CTA, read by the others
+  int* before = total + E;              // [E] assignments of earlier CTAs
+  int* all = before + E;                // [E] of the cluster
+  int* first = all + E;                 // [E] first row
+  for (int i = tid; i < warps * pitch; i += threads) hist[i] = 0;
   __syncthreads();
-  const long long per = ((a.assignments + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
-  const long long lo = warp * per, hi = min(a.assignments, lo + per);
-  int* mine = hist + warp * E;
-  for (long long base = lo; base < hi; base += 32) {
-    const long long i = base + lane;
-    const int e = expert_of<I>(a, i, hi);
-    const unsigned peers = __match_any_sync(kFull, e);
-    if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-    __syncwarp();
-  }
-  __syncthreads();
-  for (int e = tid; e < E; e += kSortThreads) {
-    int run = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = hist[w * E + e];
-      hist[w * E + e] = run;
-      run += c;
+  const long long workers = (long long)ctas * warps;
+  const long long per = ((a.assignments + workers - 1) / workers + 31) / 32 * 32;
+  const long long lo = (rank * warps + warp) * per, hi = min(a.assignments, lo + per);
+  int* mine = hist + warp * pitch;
+  for (long long base = lo; base < hi; base += 32 * AHEAD) {
+    int e[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) e[j] = expert_of<I>(a, base + 32 * j + lane, hi);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (base + 32 * j >= hi) break;
+      const unsigned peers = __match_any_sync(kFull, e[j]);
+      if (e[j] >= 0 && lane == __ffs(peers) - 1) mine[e[j]] += __popc(peers);
+      __syncwarp();
     }
-    total[e] = run;
   }
+  __syncthreads();
+  for (int e = warp; e < E; e += warps) {
+    const int c = lane < warps ? hist[lane * pitch + e] : 0;
+    const int x = inclusive_scan(c, lane);
+    if (lane < warps) hist[lane * pitch + e] = x - c;
+    if (lane == 31) total[e] = x;
+  }
+  if (ctas > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
+  for (int e = tid; e < E; e += threads) {
+    int sum = 0, earlier = 0;
+    if (ctas == 1) sum = total[e];
+    else
+      for (int r = 0; r < ctas; ++r) {
+        const int c = remote_int(total + e, r);
+        if (r < rank) earlier += c;
+        sum += c;
+      }
+    before[e] = earlier;
+    all[e] = sum;
+  }
+  if (ctas > 1) cluster_arrive();       // this CTA has read the others' totals
   __syncthreads();
   if (warp == 0) {                      // exclusive scan over the experts
     int carry = 0;
     for (int base = 0; base < E; base += 32) {
-      const int e = base + lane;
-      const int c = e < E ? total[e] : 0;
-      int x = c;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(kFull, x, off);
-        if (lane >= off) x += y;
-      }
+      const int e = base + lane, c = e < E ? all[e] : 0, x = inclusive_scan(c, lane);
       if (e < E) first[e] = carry + x - c;
       carry += __shfl_sync(kFull, x, 31);
     }
   }
   __syncthreads();
-  for (int e = tid; e < E; e += kSortThreads) {
-    a.starts[e] = a.capacity ? (int)(e * a.capacity) : first[e];
-    a.counts[e] = a.capacity && total[e] > a.capacity ? (int)a.capacity : total[e];
-  }
+  if (rank == 0)
+    for (int e = tid; e < E; e += threads) {
+      a.starts[e] = a.capacity ? (int)(e * a.capacity) : first[e];
+      a.counts[e] = a.capacity && all[e] > a.capacity ? (int)a.capacity : all[e];
+    }
   // rows without an assignment
   if (a.capacity) {
-    for (long long r = tid; r < a.rows; r += kSortThreads)
-      if (r % a.capacity >= total[r / a.capacity]) a.source[r] = -1;
+    for (int e = rank * warps + warp; e < E; e += (int)workers)
+      for (long long p = all[e] + lane; p < a.capacity; p += 32) a.source[e * a.capacity + p] = -1;
   } else {
-    for (long long r = (long long)first[E - 1] + total[E - 1] + tid; r < a.rows; r += kSortThreads) a.source[r] = -1;
+    for (long long r = (long long)first[E - 1] + all[E - 1] + rank * threads + tid; r < a.rows; r += (long long)ctas * threads)
+      a.source[r] = -1;
   }
-  for (long long base = lo; base < hi; base += 32) {
-    const long long i = base + lane;
-    const int e = expert_of<I>(a, i, hi);
-    const unsigned peers = __match_any_sync(kFull, e);
-    int place = 0;
-    if (e >= 0) place = mine[e] + __popc(peers & ((1u << lane) - 1));
-    __syncwarp();
-    if (e >= 0 && lane == __ffs(peers) - 1) mine[e] += __popc(peers);
-    __syncwarp();
-    if (i < hi) {
-      int row = -1;
-      if (e >= 0 && !(a.capacity && place >= a.capacity))
-        row = a.capacity ? (int)(e * a.capacity + place) : first[e] + place;
-      a.slot[i] = row;
-      if (row >= 0) a.source[row] = (int)i;
+  for (long long base = lo; base < hi; base += 32 * AHEAD) {
+    int e[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) e[j] = expert_of<I>(a, base + 32 * j + lane, hi);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const long long i = base + 32 * j + lane;
+      if (base + 32 * j >= hi) break;
+      const unsigned peers = __match_any_sync(kFull, e[j]);
+      int place = 0;
+      if (e[j] >= 0) place = mine[e[j]] + __popc(peers & ((1u << lane) - 1));
+      __syncwarp();
+      if (e[j] >= 0 && lane == __ffs(peers) - 1) mine[e[j]] += __popc(peers);
+      __syncwarp();
+      if (i < hi) {
+        int row = -1;
+        if (e[j] >= 0) {
+          place += before[e[j]];
+          if (a.capacity == 0) row = first[e[j]] + place;
+          else if (place < a.capacity) row = (int)(e[j] * a.capacity + place);
+        }
+        a.slot[i] = row;
+        if (row >= 0) a.source[row] = (int)i;
+      }
     }
   }
+  if (ctas > 1) cluster_wait();         // the totals stay until every CTA has read them
 }
 
 // ---- rows -----------------------------------------------------------------------------------------------
+//
+// All three kernels are bound by the bytes they move.  A warp moves a piece of 32 * kPieces vectors of one token
+// to or from the token's rows: the token's side is read or written once however many rows it has, and the piece's
+// vectors are all in flight together.  Vectors are the widest (16, 8 bytes or one element) that every address,
+// stride and row length allows; blockIdx.y is the piece, so no index is divided.  Blocks past the tokens' clear the
+// rows that have no token.
+constexpr int kPieces = 4;
+constexpr int kRowWarps = 8;
 
-// One CTA per token: the token is copied to each of its rows; the rest of the grid clears rows without a token.
+__device__ __forceinline__ uint4 zero_vec(uint4) { return make_uint4(0, 0, 0, 0); }
+__device__ __forceinline__ uint2 zero_vec(uint2) { return make_uint2(0, 0); }
+__device__ __forceinline__ unsigned zero_vec(unsigned) { return 0; }
+__device__ __forceinline__ unsigned short zero_vec(unsigned short) { return 0; }
+
+// rows of `source` without an assignment, 32 a warp; `block` counts from the first block past the tokens'
 template <typename V>
-__global__ void __launch_bounds__(256) dispatch_kernel(ExchangeRowsArgs a, long long units) {
+__device__ __forceinline__ void clear_rows(const ExchangeRowsArgs& a, V* out, long long stride, long long block, long long units) {
+  const int lane = threadIdx.x & 31;
+  const long long r0 = (block * (blockDim.x >> 5) + (threadIdx.x >> 5)) * 32;
+  const long long c0 = (long long)blockIdx.y * (32 * kPieces) + lane;
+  unsigned empty = __ballot_sync(kFull, r0 + lane < a.rows && a.source[r0 + lane] < 0);
+  while (empty) {
+    const long long r = r0 + __ffs(empty) - 1;
+    empty &= empty - 1;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (c0 + 32 * i < units) out[r * stride + c0 + 32 * i] = zero_vec(V{});
+  }
+}
+
+// V-sized vectors; strides and lengths are in vectors
+template <typename V>
+__global__ void __launch_bounds__(kRowWarps * 32) dispatch_kernel(ExchangeRowsArgs a, long long units, unsigned token_blocks) {
   const V* in = static_cast<const V*>(a.in);
   V* out = static_cast<V*>(a.out);
-  for (long long t = blockIdx.x; t < a.tokens; t += gridDim.x)
-    for (long long c = threadIdx.x; c < units; c += blockDim.x) {
-      const V v = in[t * a.in_stride + c];
-      for (int j = 0; j < a.k; ++j) {
-        const int r = a.slot[t * a.k + j];
-        if (r >= 0 && r < a.rows) out[r * a.out_stride + c] = v;
-      }
-    }
-  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x)
-    if (a.source[r] < 0)
-      for (long long c = threadIdx.x; c < units; c += blockDim.x) out[r * a.out_stride + c] = V{};
+  if (blockIdx.x >= token_blocks) { clear_rows(a, out, a.out_stride, blockIdx.x - token_blocks, units); return; }
+  const int lane = threadIdx.x & 31;
+  const long long t = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (t >= a.tokens) return;
+  const int mine = lane < a.k ? a.slot[t * a.k + lane] : -1;
+  const long long c0 = (long long)blockIdx.y * (32 * kPieces) + lane;
+  V v[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i)
+    if (c0 + 32 * i < units) v[i] = in[t * a.in_stride + c0 + 32 * i];
+  for (int j = 0; j < a.k; ++j) {
+    const int r = __shfl_sync(kFull, mine, j);
+    if (r < 0 || r >= a.rows) continue;
+    V* to = out + r * a.out_stride + c0;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (c0 + 32 * i < units) to[32 * i] = v[i];
+  }
 }
 
-// One CTA per token: its rows are summed in fp32, in the order of the choices.
-template <typename T>
-__global__ void __launch_bounds__(256) combine_kernel(ExchangeRowsArgs a) {
-  const T* in = static_cast<const T*>(a.in);
-  T* out = static_cast<T*>(a.out);
-  for (long long t = blockIdx.x; t < a.tokens; t += gridDim.x)
-    for (long long c = threadIdx.x; c < a.hidden; c += blockDim.x) {
-      float acc = 0.f;
-      for (int j = 0; j < a.k; ++j) {
-        const int r = a.slot[t * a.k + j];
-        if (r < 0 || r >= a.rows) continue;
-        acc = fmaf(a.weights ? a.weights[t * a.k + j] : 1.f, to_f(in[r * a.in_stride + c]), acc);
-      }
-      out[t * a.out_stride + c] = from_f<T>(acc);
+// a vector of N elements as floats and back, one rounding each
+template <typename T, int N> struct __align__(sizeof(T) * N) Vec { T v[N]; };
+
+// A token's rows are summed in fp32, in the order of the choices (weights nullptr: 1).  The next row's loads are
+// issued before a row is added.
+template <typename T, int N>
+__global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(ExchangeRowsArgs a, long long units) {
+  using V = Vec<T, N>;
+  const V* in = static_cast<const V*>(a.in);
+  const int lane = threadIdx.x & 31;
+  const long long t = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (t >= a.tokens) return;
+  int mine = -1;
+  float weight = 1.f;
+  if (lane < a.k) {
+    mine = a.slot[t * a.k + lane];
+    if (a.weights) weight = a.weights[t * a.k + lane];
+    if (mine >= a.rows) mine = -1;
+  }
+  const long long c0 = (long long)blockIdx.y * (32 * kPieces) + lane;
+  float acc[kPieces][N];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[i][n] = 0.f;
+  unsigned left = __ballot_sync(kFull, mine >= 0);
+  V next[kPieces];
+  auto fetch = [&](int j) {
+    const V* from = in + __shfl_sync(kFull, mine, j) * a.in_stride + c0;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (c0 + 32 * i < units) next[i] = from[32 * i];
+  };
+  if (left) fetch(__ffs(left) - 1);
+  while (left) {
+    const float w = __shfl_sync(kFull, weight, __ffs(left) - 1);
+    V v[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) v[i] = next[i];
+    left &= left - 1;
+    if (left) fetch(__ffs(left) - 1);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+      for (int n = 0; n < N; ++n) acc[i][n] = fmaf(w, to_f(v[i].v[n]), acc[i][n]);
+  }
+  V* out = static_cast<V*>(a.out) + t * a.out_stride + c0;
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i)
+    if (c0 + 32 * i < units) {
+      V v;
+#pragma unroll
+      for (int n = 0; n < N; ++n) v.v[n] = from_f<T>(acc[i][n]);
+      out[32 * i] = v;
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) combine_backward_kernel(ExchangeRowsArgs a) {
-  __shared__ float part[8];
-  const T* grad = static_cast<const T*>(a.in);
-  const T* rows = static_cast<const T*>(a.saved);
-  T* out = static_cast<T*>(a.out);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (long long t = blockIdx.x; t < a.tokens; t += gridDim.x)
-    for (int j = 0; j < a.k; ++j) {
-      const int r = a.slot[t * a.k + j];
-      const bool kept = r >= 0 && r < a.rows;
+// One CTA per token, its warps share the pieces: a piece of the gradient is read once and multiplied with and into
+// each of the token's rows.  The products of the pieces are added in a fixed order.
+template <typename T, int N>
+__global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(ExchangeRowsArgs a, long long units, unsigned token_blocks) {
+  using V = Vec<T, N>;
+  __shared__ float part[kRowWarps][kMaxChoices];
+  V* out = static_cast<V*>(a.out);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (blockIdx.x >= token_blocks) {     // 32 rows a warp, every piece of them
+    const long long r0 = ((long long)(blockIdx.x - token_blocks) * warps + warp) * 32;
+    unsigned empty = __ballot_sync(kFull, r0 + lane < a.rows && a.source[r0 + lane] < 0);
+    V zero;
+#pragma unroll
+    for (int n = 0; n < N; ++n) zero.v[n] = from_f<T>(0.f);
+    for (; empty; empty &= empty - 1)
+      for (long long c = lane; c < units; c += 32) out[(r0 + __ffs(empty) - 1) * a.out_stride + c] = zero;
+    return;
+  }
+  const long long t = blockIdx.x;
+  int mine = -1;
+  float weight = 0.f, dots = 0.f;       // lane j: choice j
+  if (lane < a.k) {
+    mine = a.slot[t * a.k + lane];
+    weight = a.weights[t * a.k + lane];
+    if (mine >= a.rows) mine = -1;
+  }
+  const unsigned kept = __ballot_sync(kFull, mine >= 0);
+  for (long long c0 = (long long)warp * (32 * kPieces) + lane; c0 - lane < units; c0 += (long long)warps * (32 * kPieces)) {
+    const V* from = static_cast<const V*>(a.in) + t * a.in_stride + c0;
+    V g[kPieces], next[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (c0 + 32 * i < units) g[i] = from[32 * i];
+    auto fetch = [&](int j) {
+      const V* row = static_cast<const V*>(a.saved) + __shfl_sync(kFull, mine, j) * a.saved_stride + c0;
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        if (c0 + 32 * i < units) next[i] = row[32 * i];
+    };
+    unsigned left = kept;
+    if (left) fetch(__ffs(left) - 1);
+    while (left) {
+      const int j = __ffs(left) - 1;
+      const float w = __shfl_sync(kFull, weight, j);
+      V* to = out + __shfl_sync(kFull, mine, j) * a.out_stride + c0;
+      V v[kPieces];
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) v[i] = next[i];
+      left &= left - 1;
+      if (left) fetch(__ffs(left) - 1);
       float dot = 0.f;
-      if (kept) {
-        const float w = a.weights[t * a.k + j];
-        for (long long c = threadIdx.x; c < a.hidden; c += blockDim.x) {
-          const float g = to_f(grad[t * a.in_stride + c]);
-          dot = fmaf(g, to_f(rows[r * a.saved_stride + c]), dot);
-          out[r * a.out_stride + c] = from_f<T>(w * g);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        if (c0 + 32 * i < units) {
+          V o;
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            const float x = to_f(g[i].v[n]);
+            dot = fmaf(x, to_f(v[i].v[n]), dot);
+            o.v[n] = from_f<T>(w * x);
+          }
+          to[32 * i] = o;
         }
-      }
       dot = warp_sum(dot);
-      if (lane == 0) part[warp] = dot;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        float sum = 0.f;
-        for (int w = 0; w < 8; ++w) sum += part[w];
-        a.grad_weights[t * a.k + j] = sum;
-      }
-      __syncthreads();
+      if (lane == j) dots += dot;
     }
-  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x)
-    if (a.source[r] < 0)
-      for (long long c = threadIdx.x; c < a.hidden; c += blockDim.x) out[r * a.out_stride + c] = from_f<T>(0.f);
-}
-
-unsigned row_grid(const ExchangeRowsArgs& a, bool rows) {
-  const long long n = rows && a.rows > a.tokens ? a.rows : a.tokens;
-  return (unsigned)(n < 1 ? 1 : n > 148 * 64 ? 148 * 64 : n);
+  }
+  part[warp][lane] = dots;
+  __syncthreads();
+  if (threadIdx.x < a.k) {
+    float sum = 0.f;
+    for (int w = 0; w < warps; ++w) sum += part[w][threadIdx.x];
+    a.grad_weights[t * a.k + threadIdx.x] = sum;
+  }
 }
 
 int elem_size(int dtype) { return dtype == DT_F32 ? 4 : 2; }
@@ -353,37 +525,112 @@ cudaError_t launch_route(const RouteArgs& a, cudaStream_t stream) { return route
 cudaError_t launch_route_backward(const RouteArgs& a, cudaStream_t stream) { return route_any<true>(a, stream); }
 
 cudaError_t launch_sort(const SortArgs& a, cudaStream_t stream) {
-  const size_t bytes = sizeof(int) * ((size_t)kSortWarps + 2) * a.experts;
+  // warps first, then CTAs, each with a run of at least kSortRun assignments
+  const long long workers = (a.assignments + kSortRun - 1) / kSortRun;
+  const int warps = workers < 1 ? 1 : workers > kSortWarps ? kSortWarps : (int)workers;
+  int ctas = 1;
+  while (ctas < kSortCtas && (long long)ctas * kSortWarps < workers) ctas *= 2;
+  const size_t bytes = sizeof(int) * ((size_t)warps * (a.experts | 1) + 4 * (size_t)a.experts);
   auto kernel = a.ids64 ? sort_kernel<long long> : sort_kernel<int>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && ctas > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
-  kernel<<<1, kSortThreads, bytes, stream>>>(a);
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(ctas);
+  config.blockDim = dim3(warps * 32);
+  config.dynamicSmemBytes = bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  config.attrs = &attr;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, a);
+}
+
+namespace {
+
+// The widest vector (16, 8 bytes or one element) of every matrix of the call, in bytes.
+int vector_bytes(const ExchangeRowsArgs& a) {
+  const int es = elem_size(a.dtype);
+  const unsigned long long bits = reinterpret_cast<uintptr_t>(a.in) | reinterpret_cast<uintptr_t>(a.out) |
+                                  reinterpret_cast<uintptr_t>(a.saved) | (unsigned long long)(a.hidden * es) |
+                                  (unsigned long long)(a.in_stride * es) | (unsigned long long)(a.out_stride * es) |
+                                  (unsigned long long)(a.saved_stride * es);
+  return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : es;
+}
+
+// strides and lengths in vectors of `per` elements; the number of pieces of a row
+long long in_vectors(ExchangeRowsArgs& a, int per) {
+  a.hidden /= per;
+  a.in_stride /= per;
+  a.out_stride /= per;
+  a.saved_stride /= per;
+  return (a.hidden + 32 * kPieces - 1) / (32 * kPieces);
+}
+
+template <typename V>
+cudaError_t dispatch_as(ExchangeRowsArgs a, cudaStream_t stream) {
+  const long long pieces = in_vectors(a, (int)sizeof(V) / elem_size(a.dtype));
+  const unsigned token_blocks = (unsigned)((a.tokens + kRowWarps - 1) / kRowWarps);
+  const unsigned clear_blocks = (unsigned)((a.rows + 32 * kRowWarps - 1) / (32 * kRowWarps));
+  if (pieces > 65535) return cudaErrorInvalidConfiguration;
+  dispatch_kernel<V><<<dim3(token_blocks + clear_blocks, (unsigned)pieces), kRowWarps * 32, 0, stream>>>(a, a.hidden, token_blocks);
   return cudaGetLastError();
 }
 
-cudaError_t launch_dispatch(const ExchangeRowsArgs& a, cudaStream_t stream) {
-  if (a.hidden == 0 || (a.rows == 0)) return cudaSuccess;
-  if (elem_size(a.dtype) == 4) dispatch_kernel<unsigned><<<row_grid(a, true), 256, 0, stream>>>(a, a.hidden);
-  else dispatch_kernel<unsigned short><<<row_grid(a, true), 256, 0, stream>>>(a, a.hidden);
+template <typename T, int N>
+cudaError_t combine_as(ExchangeRowsArgs a, cudaStream_t stream) {
+  const long long pieces = in_vectors(a, N);
+  if (pieces > 65535) return cudaErrorInvalidConfiguration;
+  const unsigned blocks = (unsigned)((a.tokens + kRowWarps - 1) / kRowWarps);
+  combine_kernel<T, N><<<dim3(blocks, (unsigned)pieces), kRowWarps * 32, 0, stream>>>(a, a.hidden);
   return cudaGetLastError();
+}
+
+template <typename T, int N>
+cudaError_t combine_backward_as(ExchangeRowsArgs a, cudaStream_t stream) {
+  const long long pieces = in_vectors(a, N);
+  const int warps = pieces < 1 ? 1 : pieces > kRowWarps ? kRowWarps : (int)pieces;
+  const unsigned clear_blocks = (unsigned)((a.rows + 32 * warps - 1) / (32 * warps));
+  if (a.tokens + clear_blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  combine_backward_kernel<T, N><<<(unsigned)a.tokens + clear_blocks, warps * 32, 0, stream>>>(a, a.hidden, (unsigned)a.tokens);
+  return cudaGetLastError();
+}
+
+template <typename T, bool BACKWARD>
+cudaError_t combine_any(const ExchangeRowsArgs& a, cudaStream_t stream) {
+  constexpr int es = (int)sizeof(T);
+  const int bytes = vector_bytes(a);
+  if (bytes == 16) return BACKWARD ? combine_backward_as<T, 16 / es>(a, stream) : combine_as<T, 16 / es>(a, stream);
+  if (bytes == 8) return BACKWARD ? combine_backward_as<T, 8 / es>(a, stream) : combine_as<T, 8 / es>(a, stream);
+  return BACKWARD ? combine_backward_as<T, 1>(a, stream) : combine_as<T, 1>(a, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_dispatch(const ExchangeRowsArgs& a, cudaStream_t stream) {
+  if (a.hidden == 0 || a.rows == 0) return cudaSuccess;
+  const int bytes = vector_bytes(a);
+  if (bytes == 16) return dispatch_as<uint4>(a, stream);
+  if (bytes == 8) return dispatch_as<uint2>(a, stream);
+  return bytes == 4 ? dispatch_as<unsigned>(a, stream) : dispatch_as<unsigned short>(a, stream);
 }
 
 cudaError_t launch_combine(const ExchangeRowsArgs& a, cudaStream_t stream) {
   if (a.hidden == 0 || a.tokens == 0) return cudaSuccess;
-  const unsigned grid = row_grid(a, false);
-  if (a.dtype == DT_F32) combine_kernel<float><<<grid, 256, 0, stream>>>(a);
-  else if (a.dtype == DT_BF16) combine_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
-  else combine_kernel<__half><<<grid, 256, 0, stream>>>(a);
-  return cudaGetLastError();
+  if (a.dtype == DT_F32) return combine_any<float, false>(a, stream);
+  if (a.dtype == DT_BF16) return combine_any<__nv_bfloat16, false>(a, stream);
+  return combine_any<__half, false>(a, stream);
 }
 
 cudaError_t launch_combine_backward(const ExchangeRowsArgs& a, cudaStream_t stream) {
   if (a.tokens == 0 && a.rows == 0) return cudaSuccess;
-  const unsigned grid = row_grid(a, true);
-  if (a.dtype == DT_F32) combine_backward_kernel<float><<<grid, 256, 0, stream>>>(a);
-  else if (a.dtype == DT_BF16) combine_backward_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(a);
-  else combine_backward_kernel<__half><<<grid, 256, 0, stream>>>(a);
-  return cudaGetLastError();
+  if (a.dtype == DT_F32) return combine_any<float, true>(a, stream);
+  if (a.dtype == DT_BF16) return combine_any<__nv_bfloat16, true>(a, stream);
+  return combine_any<__half, true>(a, stream);
 }
 
 }  // namespace vb

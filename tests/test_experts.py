@@ -328,7 +328,13 @@ def test_strided_and_broadcast_rows(dtype, hidden, offset, pitch):
     assert torch.equal(ex.combine(values, weights, order), ex.combine(values.contiguous(), weights, order))
     grads = ex.combine_backward(view, values, weights, order, out=store[:, offset:offset + hidden])
     plain = ex.combine_backward(view.contiguous(), values.contiguous(), weights, order)
-    assert torch.equal(grads[0], plain[0]) and torch.equal(grads[1], plain[1])
+    assert torch.equal(grads[0], plain[0])
+    # the order of a product's fp32 additions follows the widest vector the addresses allow, so its sums may differ
+    # by the roundings of hidden additions: both are held to the 64-bit value
+    parts = torch.where((order.slot >= 0)[..., None], values.double()[order.slot.clamp(min=0).long()], 0.0) * \
+        view.double()[:, None]
+    close(grads[1], parts.sum(2), parts.abs().sum(2), torch.float32, hidden)
+    close(plain[1], parts.sum(2), parts.abs().sum(2), torch.float32, hidden)
     assert bool((store[:, :offset] == 7).all()) and bool((store[:, offset + hidden:] == 7).all())
     one = wide[:1, offset:offset + hidden].expand(50, hidden)
     assert torch.equal(ex.dispatch(one, order), ex.dispatch(one.contiguous(), order))

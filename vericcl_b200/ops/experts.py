@@ -27,6 +27,7 @@ from vericcl_b200.ops import native
 
 MAX_EXPERTS = 1024
 MAX_CHOICES = 32
+MAX_COLUMNS = 1 << 22
 INT4_GROUPS = (32, 64, 128)
 _DTYPES = frozenset({torch.float32, torch.bfloat16, torch.float16})
 _INT_MAX = 2 ** 31 - 1
@@ -64,6 +65,8 @@ class ExpertOrder:
 def _matrix(t, name):
     if t.dim() != 2 or t.dtype not in _DTYPES:
         raise RuntimeFailure("%s must be a [rows, columns] matrix of float32, bfloat16 or float16" % name)
+    if t.size(1) > MAX_COLUMNS:
+        raise RuntimeFailure("%s has more than %d columns" % (name, MAX_COLUMNS))
     if t.size(1) > 1 and t.stride(1) != 1:
         raise RuntimeFailure("%s must have contiguous rows (stride 1 in the last dimension)" % name)
 
