@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "vb/launch.h"
@@ -532,8 +533,16 @@ cudaError_t launch_sort(const SortArgs& a, cudaStream_t stream) {
   while (ctas < kSortCtas && (long long)ctas * kSortWarps < workers) ctas *= 2;
   const size_t bytes = sizeof(int) * ((size_t)warps * (a.experts | 1) + 4 * (size_t)a.experts);
   auto kernel = a.ids64 ? sort_kernel<long long> : sort_kernel<int>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e == cudaSuccess && ctas > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  // the attributes are set once per device and index type, for the most experts
+  static std::atomic<unsigned long long> allowed[2];
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && (device >= 64 || !(allowed[a.ids64 ? 1 : 0].load() >> device & 1))) {
+    const size_t most = sizeof(int) * ((size_t)kSortWarps * (kMaxExperts | 1) + 4 * kMaxExperts);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && device < 64) allowed[a.ids64 ? 1 : 0].fetch_or(1ull << device);
+  }
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(ctas);

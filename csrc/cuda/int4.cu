@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <climits>
 #include <cstdint>
 #include <type_traits>
@@ -461,7 +462,14 @@ cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
   auto kernel = int4_product_kernel<T, S, VEC>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  // the shared-memory limit is raised once per device and instance
+  static std::atomic<unsigned long long> allowed{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && (device >= 64 || !(allowed.load() >> device & 1))) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device < 64) allowed.fetch_or(1ull << device);
+  }
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t config{};
   if (n_tiles * items * ranks > INT_MAX) return cudaErrorInvalidConfiguration;

@@ -1,10 +1,12 @@
-// Bindings of the mixture-of-experts operators.  vericcl_b200/ops/experts.py checks the arguments first and says
-// what is wrong with them; the checks here keep a direct call inside its buffers.
+// Bindings of the mixture-of-experts operators.  A call refuses whatever vericcl_b200/ops/experts.py documents as
+// refused before it launches anything; that file then says which argument was wrong.  Small calls cost what their
+// host side costs, so results are allocated and cut without going through the dispatcher.
 #include <cuda_runtime.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <climits>
@@ -29,21 +31,49 @@ int code_of(const Tensor& t) {
 }
 
 void done(cudaError_t e, const char* what) {
-  if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+  if (e == cudaSuccess) return;
+  cudaGetLastError();            // reported here, not again by the next call that looks
+  throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
+constexpr int64_t kMaxColumns = 1 << 22;
+
 // a CUDA matrix on `like`'s device whose rows are contiguous
 void check_matrix(const Tensor& t, const Tensor& like, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " is not on the call's GPU");
-  TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && t.stride(0) >= 0, name,
+  TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && t.size(1) <= kMaxColumns, name,
               " is no matrix of contiguous rows");
 }
 
 void check_table(const Tensor& t, const Tensor& like, at::ScalarType type, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.is_contiguous() && t.scalar_type() == type, name,
               " is not a contiguous table of its type on the call's GPU");
+}
+
+// the bytes from a matrix's first element to its last
+std::pair<const char*, const char*> span(const Tensor& t) {
+  const char* lo = static_cast<const char*>(t.data_ptr());
+  return {lo, t.numel() ? lo + ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size() : lo};
+}
+
+void check_apart(const Tensor& out, const Tensor& in) {
+  const auto a = span(out), b = span(in);
+  TORCH_CHECK(a.first >= b.second || b.first >= a.second, "out overlaps an input");
+}
+
+Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
+// a contiguous tensor of `type` (4 bytes an element) inside the int32 tensor `pool`, from element `offset` on
+Tensor cut(const Tensor& pool, int64_t offset, at::IntArrayRef sizes, at::ScalarType type = at::kInt) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(pool.storage()), pool.key_set(),
+                                                    at::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  t.unsafeGetTensorImpl()->set_storage_offset(offset);
+  return t;
 }
 
 void check_order(const Tensor& slot, const Tensor& source, const Tensor& like) {
@@ -69,21 +99,25 @@ ExchangeRowsArgs row_args(const Tensor& in, const Tensor& out, const Tensor& slo
   return a;
 }
 
-Tensor made(const std::optional<Tensor>& out, int64_t rows, const Tensor& like) {
-  if (!out) return at::empty({rows, like.size(1)}, like.options());
+// the result [rows, columns] of `like`'s dtype: a new tensor, or `out` if it is one of that kind, away from `like`
+Tensor made(const std::optional<Tensor>& out, int64_t rows, int64_t columns, const Tensor& like) {
+  if (!out) return empty({rows, columns}, like.scalar_type(), like);
   check_matrix(*out, like, "out");
-  TORCH_CHECK(out->size(0) == rows && out->size(1) == like.size(1) && out->scalar_type() == like.scalar_type(),
+  TORCH_CHECK(out->size(0) == rows && out->size(1) == columns && out->scalar_type() == like.scalar_type(),
               "out has another shape or dtype than the result");
-  TORCH_CHECK(out->size(0) <= 1 || out->stride(0) >= out->size(1), "out's rows overlap");
+  TORCH_CHECK(rows <= 1 || out->stride(0) >= columns, "out's rows overlap");
+  check_apart(*out, like);
   return *out;
 }
 
 py::tuple route(const Tensor& logits, int64_t k, bool renormalize) {
   check_matrix(logits, logits, "logits");
-  TORCH_CHECK(k >= 1 && k <= kMaxChoices && k <= logits.size(1) && logits.size(1) <= kMaxExperts, "bad k or experts");
+  TORCH_CHECK(k >= 1 && k <= kMaxChoices && k <= logits.size(1) && logits.size(1) <= kMaxExperts &&
+              logits.size(0) * k <= INT_MAX, "bad k, experts or tokens");
   c10::cuda::CUDAGuard guard(logits.device());
-  auto ids = at::empty({logits.size(0), k}, logits.options().dtype(at::kInt));
-  auto weights = at::empty({logits.size(0), k}, logits.options().dtype(at::kFloat));
+  const int64_t n = logits.size(0) * k, sizes[2] = {logits.size(0), k};
+  auto pool = empty({2 * n}, at::kInt, logits);
+  auto ids = cut(pool, 0, sizes), weights = cut(pool, n, sizes, at::kFloat);
   RouteArgs a{};
   a.logits = logits.data_ptr();
   a.logits_stride = logits.stride(0);
@@ -104,11 +138,11 @@ Tensor route_backward(const Tensor& logits, const Tensor& ids, const Tensor& wei
   check_table(ids, logits, at::kInt, "ids");
   check_table(weights, logits, at::kFloat, "weights");
   check_table(grad, logits, at::kFloat, "grad_weights");
-  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == logits.size(0) && ids.size(1) <= kMaxChoices &&
-              weights.sizes() == ids.sizes() && grad.sizes() == ids.sizes() && logits.size(1) <= kMaxExperts,
+  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == logits.size(0) && ids.size(1) >= 1 && ids.size(1) <= kMaxChoices &&
+              ids.size(1) <= logits.size(1) && ids.numel() <= INT_MAX && weights.sizes() == ids.sizes() && grad.sizes() == ids.sizes() && logits.size(1) <= kMaxExperts,
               "ids, weights and grad_weights are [tokens, k]");
   c10::cuda::CUDAGuard guard(logits.device());
-  auto out = at::empty({logits.size(0), logits.size(1)}, logits.options());
+  auto out = empty({logits.size(0), logits.size(1)}, logits.scalar_type(), logits);
   RouteArgs a{};
   a.logits = logits.data_ptr();
   a.logits_stride = logits.stride(0);
@@ -128,16 +162,16 @@ Tensor route_backward(const Tensor& logits, const Tensor& ids, const Tensor& wei
 py::tuple sort_by_expert(const Tensor& ids, int64_t experts, int64_t capacity) {
   TORCH_CHECK(ids.is_cuda() && ids.is_contiguous() && ids.dim() == 2 &&
               (ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong), "ids are contiguous int32 or int64");
-  TORCH_CHECK(experts >= 1 && experts <= kMaxExperts && capacity >= 0 && capacity <= INT_MAX, "bad experts or capacity");
+  TORCH_CHECK(experts >= 1 && experts <= kMaxExperts && capacity >= 0 && capacity <= INT_MAX && ids.size(1) >= 1 &&
+              ids.size(1) <= kMaxChoices, "bad experts, capacity or choices");
   const int64_t rows = capacity ? experts * capacity : ids.numel();
   TORCH_CHECK(ids.numel() <= INT_MAX && rows <= INT_MAX, "more than 2^31 - 1 assignments or rows");
   c10::cuda::CUDAGuard guard(ids.device());
   // one allocation for the four tables
-  auto pool = at::empty({ids.numel() + rows + 2 * experts}, ids.options().dtype(at::kInt));
-  auto slot = pool.narrow(0, 0, ids.numel()).view(ids.sizes());
-  auto source = pool.narrow(0, ids.numel(), rows);
-  auto counts = pool.narrow(0, ids.numel() + rows, experts);
-  auto starts = pool.narrow(0, ids.numel() + rows + experts, experts);
+  const int64_t n = ids.numel();
+  auto pool = empty({n + rows + 2 * experts}, at::kInt, ids);
+  auto slot = cut(pool, 0, ids.sizes()), source = cut(pool, n, {rows});
+  auto counts = cut(pool, n + rows, {experts}), starts = cut(pool, n + rows + experts, {experts});
   SortArgs a{};
   a.ids = ids.data_ptr();
   a.ids64 = ids.scalar_type() == at::kLong ? 1 : 0;
@@ -158,7 +192,7 @@ Tensor dispatch(const Tensor& x, const Tensor& slot, const Tensor& source, const
   check_order(slot, source, x);
   TORCH_CHECK(x.size(0) == slot.size(0), "x has another number of tokens than the order");
   c10::cuda::CUDAGuard guard(x.device());
-  auto rows = made(out, source.numel(), x);
+  auto rows = made(out, source.numel(), x.size(1), x);
   done(launch_dispatch(row_args(x, rows, slot, source), stream()), "dispatch launch");
   return rows;
 }
@@ -169,7 +203,7 @@ Tensor combine(const Tensor& rows, const std::optional<Tensor>& weights, const T
   check_order(slot, source, rows);
   TORCH_CHECK(rows.size(0) == source.numel(), "rows has another number of rows than the order");
   c10::cuda::CUDAGuard guard(rows.device());
-  auto tokens = made(out, slot.size(0), rows);
+  auto tokens = made(out, slot.size(0), rows.size(1), rows);
   auto a = row_args(rows, tokens, slot, source);
   if (weights) {
     check_table(*weights, rows, at::kFloat, "weights");
@@ -190,8 +224,9 @@ py::tuple combine_backward(const Tensor& grad, const Tensor& rows, const Tensor&
               rows.scalar_type() == grad.scalar_type() && weights.sizes() == slot.sizes(),
               "grad_out, rows, weights and the order do not fit together");
   c10::cuda::CUDAGuard guard(grad.device());
-  auto grad_rows = made(out, source.numel(), grad);
-  auto grad_weights = at::empty(slot.sizes(), weights.options());
+  auto grad_rows = made(out, source.numel(), grad.size(1), grad);
+  if (out) check_apart(*out, rows);
+  auto grad_weights = empty(slot.sizes(), at::kFloat, grad);
   auto a = row_args(grad, grad_rows, slot, source);
   a.saved = rows.data_ptr();
   a.saved_stride = rows.stride(0);
@@ -221,15 +256,8 @@ Tensor int4_product(const Tensor& x, const Tensor& starts, const Tensor& counts,
               "more than 2^31 - 1 rows, weight rows or inner values");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 == 0, "packed starts on a 16-byte boundary");
   c10::cuda::CUDAGuard guard(x.device());
-  Tensor y;
-  if (out) {
-    y = *out;
-    check_matrix(y, x, "out");
-    TORCH_CHECK(y.size(0) == x.size(0) && y.size(1) == packed.size(1) && y.scalar_type() == x.scalar_type() &&
-                (y.size(0) <= 1 || y.stride(0) >= y.size(1)), "out is [rows, n] of the rows' dtype");
-  } else {
-    y = at::empty({x.size(0), packed.size(1)}, x.options());
-  }
+  TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()), "4-bit products have no gradient");
+  auto y = made(out, x.size(0), packed.size(1), x);
   Int4Args a{};
   a.x = x.data_ptr();
   a.x_stride = x.stride(0);

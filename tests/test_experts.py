@@ -33,7 +33,7 @@ def _cpu_order(tokens=3, k=2, rows=6):
                           torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
 
 
-@pytest.mark.parametrize("call", [
+REFUSED = [
     lambda: ex.route(torch.zeros(3), 1),
     lambda: ex.route(torch.zeros(3, 4, dtype=torch.float64), 1),
     lambda: ex.route(torch.zeros(3, 4), 0),
@@ -71,10 +71,33 @@ def _cpu_order(tokens=3, k=2, rows=6):
     lambda: ex.quantize_int4(torch.zeros(8, 100), 32),
     lambda: ex.quantize_int4(torch.zeros(8, 96), 48),
     lambda: ex.quantize_int4(torch.zeros(8, 128), 128, scale_dtype=torch.float64),
-])
+]
+
+
+@pytest.mark.parametrize("call", REFUSED)
 def test_refusals(call):
     with pytest.raises(RuntimeFailure):
         call()
+
+
+@pytest.mark.gpu
+def test_the_same_calls_are_refused_on_the_gpu():
+    cuda()
+    for call in REFUSED:
+        with torch.device("cuda"), pytest.raises(RuntimeFailure):
+            call()
+    for change in PRODUCT_REFUSED:
+        with pytest.raises(RuntimeFailure):
+            # a view that starts off the 16-byte grid stays one
+            ex.expert_matmul_int4(**{k: on_gpu(v) for k, v in _product_args(**change).items()})
+    with pytest.raises(RuntimeFailure, match="different devices"):
+        ex.dispatch(torch.zeros(3, 8, device="cuda"), _cpu_order())
+
+
+def on_gpu(t):
+    return t.detach().cuda().as_strided(t.shape, t.stride()).requires_grad_(t.requires_grad) if t.is_contiguous() and \
+        t.storage_offset() == 0 else torch.empty(t.untyped_storage().nbytes() // t.element_size(), dtype=t.dtype,
+                                                 device="cuda").as_strided(t.shape, t.stride(), t.storage_offset())
 
 
 def _product_args(**change):
@@ -85,7 +108,7 @@ def _product_args(**change):
     return args
 
 
-@pytest.mark.parametrize("change", [
+PRODUCT_REFUSED = [
     dict(rows=torch.zeros(5, 128)), dict(rows=torch.zeros(5, 126, dtype=torch.bfloat16)),
     dict(rows=torch.zeros(128, 5, dtype=torch.bfloat16).t()),
     dict(starts=torch.zeros(3, dtype=torch.int32)), dict(starts=torch.zeros(2, dtype=torch.int64)),
@@ -101,7 +124,10 @@ def _product_args(**change):
     dict(scales=torch.zeros(2, 8, 1, dtype=torch.bfloat16)),
     dict(rows=torch.zeros(5, 128, dtype=torch.bfloat16, requires_grad=True)),
     dict(out=torch.zeros(5, 8, dtype=torch.bfloat16)), dict(out=torch.zeros(5, 7, dtype=torch.float16)),
-])
+]
+
+
+@pytest.mark.parametrize("change", PRODUCT_REFUSED)
 def test_product_refusals(change):
     with pytest.raises(RuntimeFailure):
         ex.expert_matmul_int4(**_product_args(**change))

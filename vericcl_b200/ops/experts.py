@@ -42,6 +42,21 @@ def _mod():
     return _module
 
 
+def _call(name, check, *args):
+    """The native call ``name(*args)``, which refuses bad arguments before it launches anything; ``check()`` then says
+    what was wrong.  Tensors off the GPU never reach it."""
+    if args[0].is_cuda:
+        try:
+            return getattr(_module or _mod(), name)(*args)
+        except torch.OutOfMemoryError:
+            raise
+        except (RuntimeError, TypeError) as error:
+            check()
+            raise RuntimeFailure("%s: %s" % (name, str(error).splitlines()[0])) from error
+    check()
+    raise RuntimeFailure("the expert operators need CUDA tensors")
+
+
 class ExpertOrder:
     """Where each assignment's row is: the result of :func:`sort_by_expert`.
 
@@ -118,10 +133,11 @@ def _apart(out, name, *inputs):
             raise RuntimeFailure("%s overlaps an input" % name)
 
 
-def _learns(*tensors) -> bool:
-    if not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors):
+def _learns() -> bool:
+    """Whether an input that requires a gradient is recorded by autograd."""
+    if not torch.is_grad_enabled():
         return False
-    if torch.cuda.is_current_stream_capturing():
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         raise RuntimeFailure("autograd under graph capture: capture the plain calls (detached inputs and the "
                              "*_backward functions) instead")
     return True
@@ -147,6 +163,7 @@ def _check_route(logits, k):
         raise RuntimeFailure("k must be 1 to min(%d, experts)" % MAX_CHOICES)
     if logits.size(0) * logits.size(1) > 2 ** 40 or logits.size(0) * k > _INT_MAX:
         raise RuntimeFailure("more than 2^31 - 1 assignments")
+    _on_gpu(logits)
 
 
 def route(logits: torch.Tensor, k: int, *, renormalize: bool = True):
@@ -157,28 +174,27 @@ def route(logits: torch.Tensor, k: int, *, renormalize: bool = True):
     A logit of -inf takes its expert out: a token with fewer than ``k`` experts left gets id -1 and weight 0 for
     the rest.  A NaN logit is never chosen and makes the weights of its token NaN.
     """
-    _check_route(logits, k)
-    _on_gpu(logits)
-    if _learns(logits):
+    if logits.requires_grad and _learns():
         return _Route.apply(logits, k, renormalize)
-    return _mod().route(logits, k, renormalize)
+    return _call("route", lambda: _check_route(logits, k), logits, k, renormalize)
 
 
 def route_backward(logits, ids, weights, grad_weights, *, renormalize: bool = True) -> torch.Tensor:
     """Gradient of ``route``'s weights with respect to ``logits`` [tokens, experts], in the logits' dtype."""
-    _check_route(logits, ids.size(-1) if ids.dim() else 0)
-    shape = (logits.size(0), ids.size(-1))
-    _table(ids, shape, torch.int32, "ids")
-    _table(weights, shape, torch.float32, "weights")
-    _table(grad_weights, shape, torch.float32, "grad_weights")
-    _on_gpu(logits, ids, weights, grad_weights)
-    return _mod().route_backward(logits, ids, weights, grad_weights, renormalize)
+    def check():
+        shape = (logits.size(0) if logits.dim() else 0, ids.size(-1) if ids.dim() else 0)
+        _table(ids, shape, torch.int32, "ids")
+        _table(weights, shape, torch.float32, "weights")
+        _table(grad_weights, shape, torch.float32, "grad_weights")
+        _check_route(logits, shape[1])
+        _on_gpu(logits, ids, weights, grad_weights)
+    return _call("route_backward", check, logits, ids, weights, grad_weights, renormalize)
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, renormalize):
-        ids, weights = _mod().route(logits, k, renormalize)
+        ids, weights = _call("route", lambda: _check_route(logits, k), logits, k, renormalize)
         ctx.renormalize = renormalize
         ctx.save_for_backward(logits, ids, weights)
         ctx.mark_non_differentiable(ids)
@@ -187,8 +203,7 @@ class _Route(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, _, grad):
-        logits, ids, weights = ctx.saved_tensors
-        return _mod().route_backward(logits, ids, weights, grad.contiguous(), ctx.renormalize), None, None
+        return route_backward(*ctx.saved_tensors, grad.contiguous(), renormalize=ctx.renormalize), None, None
 
 
 # -- sort, dispatch, combine ------------------------------------------------------------------------------
@@ -201,18 +216,19 @@ def sort_by_expert(ids: torch.Tensor, experts: int, *, capacity: int | None = No
     it expert ``e`` owns the rows ``e * capacity ... (e + 1) * capacity - 1`` and assignments beyond them have
     none.  An id outside ``[0, experts)`` (-1 for a padded token) has no row.
     """
-    if ids.dim() != 2 or ids.dtype not in (torch.int32, torch.int64) or not ids.is_contiguous():
-        raise RuntimeFailure("ids must be a contiguous int32 or int64 tensor [tokens, k]")
-    if not 1 <= experts <= MAX_EXPERTS:
-        raise RuntimeFailure("1 to %d experts" % MAX_EXPERTS)
-    if capacity is not None and capacity < 1:
-        raise RuntimeFailure("a capacity is at least one row per expert")
-    if ids.size(1) < 1 or ids.size(1) > MAX_CHOICES:
-        raise RuntimeFailure("1 to %d choices per token" % MAX_CHOICES)
-    if ids.numel() > _INT_MAX or experts * (capacity or 0) > _INT_MAX:
-        raise RuntimeFailure("more than 2^31 - 1 assignments or rows")
-    _on_gpu(ids)
-    return ExpertOrder(*_mod().sort_by_expert(ids, experts, capacity or 0))
+    def check():
+        if ids.dim() != 2 or ids.dtype not in (torch.int32, torch.int64) or not ids.is_contiguous():
+            raise RuntimeFailure("ids must be a contiguous int32 or int64 tensor [tokens, k]")
+        if not 1 <= experts <= MAX_EXPERTS:
+            raise RuntimeFailure("1 to %d experts" % MAX_EXPERTS)
+        if capacity is not None and capacity < 1:
+            raise RuntimeFailure("a capacity is at least one row per expert")
+        if ids.size(1) < 1 or ids.size(1) > MAX_CHOICES:
+            raise RuntimeFailure("1 to %d choices per token" % MAX_CHOICES)
+        if ids.numel() > _INT_MAX or experts * (capacity or 0) > _INT_MAX:
+            raise RuntimeFailure("more than 2^31 - 1 assignments or rows")
+    # a capacity of 0 would mean none to the native call
+    return ExpertOrder(*_call("sort_by_expert", check, ids, experts, 0 if capacity is None else capacity or -1))
 
 
 def _check_dispatch(x, order, out, name):
@@ -223,7 +239,6 @@ def _check_dispatch(x, order, out, name):
     _result(out, source.numel(), x, "out")
     _on_gpu(x, slot, source, out)
     _apart(out, "out", x)
-    return slot, source
 
 
 def _check_combine(rows, weights, order, out, name):
@@ -236,74 +251,73 @@ def _check_combine(rows, weights, order, out, name):
     _result(out, slot.size(0), rows, "out")
     _on_gpu(rows, slot, source, weights, out)
     _apart(out, "out", rows)
-    return slot, source
 
 
 def dispatch(x: torch.Tensor, order: ExpertOrder, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """``rows[r] = x[token of row r]`` [rows, hidden]; a row without an assignment is zero."""
-    slot, source = _check_dispatch(x, order, out, "x")
-    if _learns(x):
+    if x.requires_grad and _learns():
         _no_out(out)
-        return _Dispatch.apply(x, slot, source)
-    return _mod().dispatch(x, slot, source, out)
+        return _Dispatch.apply(x, order)
+    return _call("dispatch", lambda: _check_dispatch(x, order, out, "x"), x, order.slot, order.source, out)
 
 
 def dispatch_backward(grad_rows: torch.Tensor, order: ExpertOrder, *, out: torch.Tensor | None = None):
     """Gradient of :func:`dispatch` with respect to ``x``: the sum of each token's rows, in fp32, rounded once."""
-    slot, source = _check_combine(grad_rows, None, order, out, "grad_rows")
-    return _mod().combine(grad_rows, None, slot, source, out)
+    return _call("combine", lambda: _check_combine(grad_rows, None, order, out, "grad_rows"), grad_rows, None,
+                 order.slot, order.source, out)
 
 
 def combine(rows: torch.Tensor, weights: torch.Tensor, order: ExpertOrder, *, out: torch.Tensor | None = None):
     """``out[t] = sum over j of weights[t, j] * rows[slot[t, j]]`` [tokens, hidden], summed in fp32 in the order of
     the choices and rounded once.  An assignment without a row adds nothing, whatever its weight; ``weights`` is
     float32 [tokens, k]."""
-    slot, source = _check_combine(rows, weights, order, out, "rows")
-    if _learns(rows, weights):
+    if (rows.requires_grad or weights.requires_grad) and _learns():
         _no_out(out)
-        return _Combine.apply(rows, weights, slot, source)
-    return _mod().combine(rows, weights, slot, source, out)
+        return _Combine.apply(rows, weights, order)
+    return _call("combine", lambda: _check_combine(rows, weights, order, out, "rows"), rows, weights, order.slot,
+                 order.source, out)
 
 
 def combine_backward(grad_out, rows, weights, order: ExpertOrder, *, out: torch.Tensor | None = None):
     """``(grad_rows, grad_weights)`` of :func:`combine`: ``w * grad_out[t]`` at each assignment's row (zero in rows
     without one; written to ``out`` where given) and the fp32 products ``<grad_out[t], rows[slot]>``, zero where an
     assignment has no row."""
-    slot, source = _check_dispatch(grad_out, order, out, "grad_out")
-    _matrix(rows, "rows")
-    if tuple(rows.shape) != (source.numel(), grad_out.size(1)) or rows.dtype != grad_out.dtype:
-        raise RuntimeFailure("rows must be [%d, %d] of %s" % (source.numel(), grad_out.size(1), grad_out.dtype))
-    _table(weights, slot.shape, torch.float32, "weights")
-    _on_gpu(grad_out, rows, weights)
-    _apart(out, "out", rows)
-    return _mod().combine_backward(grad_out, rows, weights, slot, source, out)
+    def check():
+        _check_dispatch(grad_out, order, out, "grad_out")
+        _matrix(rows, "rows")
+        if tuple(rows.shape) != (order.source.numel(), grad_out.size(1)) or rows.dtype != grad_out.dtype:
+            raise RuntimeFailure("rows must be [%d, %d] of %s" % (order.source.numel(), grad_out.size(1), grad_out.dtype))
+        _table(weights, order.slot.shape, torch.float32, "weights")
+        _on_gpu(grad_out, rows, weights)
+        _apart(out, "out", rows)
+    return _call("combine_backward", check, grad_out, rows, weights, order.slot, order.source, out)
 
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, slot, source):
-        ctx.save_for_backward(slot, source)
-        return _mod().dispatch(x, slot, source, None)
+    def forward(ctx, x, order):
+        rows = dispatch(x.detach(), order)
+        ctx.save_for_backward(order.slot, order.source)
+        return rows
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        slot, source = ctx.saved_tensors
-        return _mod().combine(_rows_of(grad), None, slot, source, None), None, None
+        return dispatch_backward(_rows_of(grad), ExpertOrder(*ctx.saved_tensors, None, None)), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, weights, slot, source):
-        ctx.save_for_backward(rows, weights, slot, source)
-        return _mod().combine(rows, weights, slot, source, None)
+    def forward(ctx, rows, weights, order):
+        out = combine(rows.detach(), weights.detach(), order)
+        ctx.save_for_backward(rows, weights, order.slot, order.source)
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         rows, weights, slot, source = ctx.saved_tensors
-        grad_rows, grad_weights = _mod().combine_backward(_rows_of(grad), rows, weights, slot, source, None)
-        return grad_rows, grad_weights, None, None
+        return *combine_backward(_rows_of(grad), rows, weights, ExpertOrder(slot, source, None, None)), None
 
 
 # -- 4-bit products ---------------------------------------------------------------------------------------
@@ -329,17 +343,7 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, scale_dtype: torch.
     return (q[..., 0::2] | (q[..., 1::2] << 4)).contiguous(), scales.contiguous()
 
 
-def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, packed: torch.Tensor,
-                       scales: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
-    """``out[r] = W[e] @ rows[r]`` [rows, n] for the rows ``starts[s] ... starts[s] + counts[s] - 1`` of every
-    segment ``s``, whose expert is ``e = s % experts``; a row no segment covers is zero.
-
-    ``rows`` [rows, inner] is bfloat16 or float16; ``starts`` and ``counts`` int32 [segments] (an order's, or one
-    segment per source rank and expert after an AllToAll), a multiple of the experts, at most 1024, that ascend
-    and do not overlap; ``packed`` uint8 [experts, n, inner / 2] and ``scales`` [experts, n, inner / group] of the
-    rows' dtype or float32, as :func:`quantize_int4` gives them, in groups of 32, 64 or 128.  Products and sums are
-    fp32, rounded once.  No gradients: 4-bit weights are for serving.
-    """
+def _check_product(rows, starts, counts, packed, scales, out):
     _matrix(rows, "rows")
     if rows.dtype == torch.float32:
         raise RuntimeFailure("rows must be bfloat16 or float16")
@@ -365,4 +369,18 @@ def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.T
     _result(out, rows.size(0), rows, "out", packed.size(1))
     _on_gpu(rows, starts, counts, packed, scales, out)
     _apart(out, "out", rows)
-    return _mod().int4_product(rows, starts, counts, packed, scales, out)
+
+
+def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, packed: torch.Tensor,
+                       scales: torch.Tensor, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[r] = W[e] @ rows[r]`` [rows, n] for the rows ``starts[s] ... starts[s] + counts[s] - 1`` of every
+    segment ``s``, whose expert is ``e = s % experts``; a row no segment covers is zero.
+
+    ``rows`` [rows, inner] is bfloat16 or float16; ``starts`` and ``counts`` int32 [segments] (an order's, or one
+    segment per source rank and expert after an AllToAll), a multiple of the experts, at most 1024, that ascend
+    and do not overlap; ``packed`` uint8 [experts, n, inner / 2] and ``scales`` [experts, n, inner / group] of the
+    rows' dtype or float32, as :func:`quantize_int4` gives them, in groups of 32, 64 or 128.  Products and sums are
+    fp32, rounded once.  No gradients: 4-bit weights are for serving.
+    """
+    return _call("int4_product", lambda: _check_product(rows, starts, counts, packed, scales, out), rows, starts, counts,
+                 packed, scales, out)
