@@ -182,13 +182,25 @@ cudaError_t route_any(const RouteArgs& a, cudaStream_t stream) {
 // ---- stable sort by expert ------------------------------------------------------------------------------
 //
 // One cluster of 1 to 16 CTAs; every warp owns a contiguous run of assignments.  Pass 1 counts each warp's
-// assignments per expert (the lanes that hold one expert elect a leader with match_any, so no count depends on the
-// order of atomics), scans over the warps, over the CTAs (through distributed shared memory) and over the experts
+// assignments per expert (the lanes that hold one expert find each other by a vote per bit of the expert's number
+// and elect a leader, so no count depends on the order of atomics), scans over the warps, over the CTAs (through distributed shared memory) and over the experts
 // turn the counts into each warp's first place per expert, pass 2 hands the places out in the order of the
 // assignments.  One launch and no workspace: what it costs is the latency of these steps, not its few bytes.
 constexpr int kSortWarps = 32;         // most warps of a CTA
 constexpr int kSortCtas = 16;          // most CTAs of the cluster
 constexpr int kSortRun = 128;          // assignments of a warp before another warp or CTA is added
+
+// The lanes that hold the same expert: a vote per bit.  (match_any does this in one instruction, but sorting 131072
+// assignments to 128 experts took 23.5 us with it and takes 17.9 with the votes.)
+__device__ __forceinline__ unsigned same_expert(int e, int bits) {
+  unsigned peers = kFull;
+#pragma unroll 1
+  for (int b = 0; b < bits; ++b) {
+    const unsigned votes = __ballot_sync(kFull, e >> b & 1);
+    peers &= e >> b & 1 ? votes : ~votes;
+  }
+  return peers;
+}
 
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
@@ -233,6 +245,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
   const int E = a.experts, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int threads = blockDim.x, warps = threads >> 5, pitch = E | 1;   // an odd pitch: a column meets all banks
   const int rank = (int)cluster_rank(), ctas = (int)cluster_size();
+  const int bits = 33 - __clz(E);       // -1, no expert, has every bit set: one bit more than an expert's number
   int* hist = sm;                       // [warps][pitch] counts, then first places
   int* total = sm + warps * pitch;      // [E] of this CTA, read by the others
   int* before = total + E;              // [E] assignments of earlier CTAs
@@ -251,7 +264,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       if (base + 32 * j >= hi) break;
-      const unsigned peers = __match_any_sync(kFull, e[j]);
+      const unsigned peers = same_expert(e[j], bits);
       if (e[j] >= 0 && lane == __ffs(peers) - 1) mine[e[j]] += __popc(peers);
       __syncwarp();
     }
@@ -308,7 +321,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
     for (int j = 0; j < AHEAD; ++j) {
       const long long i = base + 32 * j + lane;
       if (base + 32 * j >= hi) break;
-      const unsigned peers = __match_any_sync(kFull, e[j]);
+      const unsigned peers = same_expert(e[j], bits);
       int place = 0;
       if (e[j] >= 0) place = mine[e[j]] + __popc(peers & ((1u << lane) - 1));
       __syncwarp();
@@ -331,13 +344,44 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
 
 // ---- rows -----------------------------------------------------------------------------------------------
 //
-// All three kernels are bound by the bytes they move.  A warp moves a piece of 32 * kPieces vectors of one token
+// All three kernels are bound by the bytes they move.  A warp moves a piece of 2 or 4 vectors a lane of one token
 // to or from the token's rows: the token's side is read or written once however many rows it has, and the piece's
 // vectors are all in flight together.  Vectors are the widest (16, 8 bytes or one element) that every address,
 // stride and row length allows; blockIdx.y is the piece, so no index is divided.  Blocks past the tokens' clear the
 // rows that have no token.
-constexpr int kPieces = 4;
+//
+// A piece is 1 KB of 16-byte vectors.  Longer pieces, or rows requested ahead, cost registers and with them the
+// warps that hide the latency: combining 8192 tokens x 8 rows x 2048 bf16 takes 53.7 us with 2 vectors a lane, 62.2
+// with 4 and 70.3 with 2 and a row ahead; dispatching 256 x 8 x 4096 takes 4.7 us with 2 and 6.0 with 4.  Shorter
+// vectors take 4 a lane (fp32 rows of 1030: dispatch 22.0 us, with 2 23.2).
+//
+// Rows that together exceed half of the L2 are read and written as streams (evicted first), as they will not be
+// found there again: 8192 x 8 x 2048 bf16 dispatch 50.9 -> 46.9 us, combine 53.7 -> 46.8, its gradient 109 -> 105.
+// Smaller ones stay for the kernel that follows.
+template <int BYTES> constexpr int kPieces = BYTES == 16 ? 2 : 4;
 constexpr int kRowWarps = 8;
+constexpr long long kStreamBytes = 64ll << 20;
+
+template <int BYTES> struct Word;
+template <> struct Word<16> { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<4> { using type = unsigned; };
+template <> struct Word<2> { using type = unsigned short; };
+
+template <bool STREAM, typename V>
+__device__ __forceinline__ V load_row(const V* p) {
+  using W = typename Word<sizeof(V)>::type;
+  const W w = STREAM ? __ldcs(reinterpret_cast<const W*>(p)) : *reinterpret_cast<const W*>(p);
+  return *reinterpret_cast<const V*>(&w);
+}
+
+template <bool STREAM, typename V>
+__device__ __forceinline__ void store_row(V* p, const V& v) {
+  using W = typename Word<sizeof(V)>::type;
+  const W w = *reinterpret_cast<const W*>(&v);
+  if (STREAM) __stcs(reinterpret_cast<W*>(p), w);
+  else *reinterpret_cast<W*>(p) = w;
+}
 
 __device__ __forceinline__ uint4 zero_vec(uint4) { return make_uint4(0, 0, 0, 0); }
 __device__ __forceinline__ uint2 zero_vec(uint2) { return make_uint2(0, 0); }
@@ -349,19 +393,20 @@ template <typename V>
 __device__ __forceinline__ void clear_rows(const ExchangeRowsArgs& a, V* out, long long stride, long long block, long long units) {
   const int lane = threadIdx.x & 31;
   const long long r0 = (block * (blockDim.x >> 5) + (threadIdx.x >> 5)) * 32;
-  const long long c0 = (long long)blockIdx.y * (32 * kPieces) + lane;
+  constexpr int P = kPieces<sizeof(V)>;
+  const long long c0 = (long long)blockIdx.y * (32 * P) + lane;
   unsigned empty = __ballot_sync(kFull, r0 + lane < a.rows && a.source[r0 + lane] < 0);
   while (empty) {
     const long long r = r0 + __ffs(empty) - 1;
     empty &= empty - 1;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i)
+    for (int i = 0; i < P; ++i)
       if (c0 + 32 * i < units) out[r * stride + c0 + 32 * i] = zero_vec(V{});
   }
 }
 
 // V-sized vectors; strides and lengths are in vectors
-template <typename V>
+template <typename V, bool STREAM>
 __global__ void __launch_bounds__(kRowWarps * 32) dispatch_kernel(ExchangeRowsArgs a, long long units, unsigned token_blocks) {
   const V* in = static_cast<const V*>(a.in);
   V* out = static_cast<V*>(a.out);
@@ -370,30 +415,29 @@ __global__ void __launch_bounds__(kRowWarps * 32) dispatch_kernel(ExchangeRowsAr
   const long long t = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   if (t >= a.tokens) return;
   const int mine = lane < a.k ? a.slot[t * a.k + lane] : -1;
-  const long long c0 = (long long)blockIdx.y * (32 * kPieces) + lane;
-  V v[kPieces];
+  constexpr int P = kPieces<sizeof(V)>;
+  const long long c0 = (long long)blockIdx.y * (32 * P) + lane;
+  V v[P];
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i)
+  for (int i = 0; i < P; ++i)
     if (c0 + 32 * i < units) v[i] = in[t * a.in_stride + c0 + 32 * i];
   for (int j = 0; j < a.k; ++j) {
     const int r = __shfl_sync(kFull, mine, j);
     if (r < 0 || r >= a.rows) continue;
     V* to = out + r * a.out_stride + c0;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-      if (c0 + 32 * i < units) to[32 * i] = v[i];
+    for (int i = 0; i < P; ++i)
+      if (c0 + 32 * i < units) store_row<STREAM>(to + 32 * i, v[i]);
   }
 }
 
-// a vector of N elements as floats and back, one rounding each
 template <typename T, int N> struct __align__(sizeof(T) * N) Vec { T v[N]; };
 
-// A token's rows are summed in fp32, in the order of the choices (weights nullptr: 1).  The next row's loads are
-// issued before a row is added.
-template <typename T, int N>
+// A token's rows are summed in fp32, in the order of the choices (weights nullptr: 1).
+template <typename T, int N, bool STREAM>
 __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(ExchangeRowsArgs a, long long units) {
   using V = Vec<T, N>;
-  const V* in = static_cast<const V*>(a.in);
+  constexpr int P = kPieces<sizeof(V)>;
   const int lane = threadIdx.x & 31;
   const long long t = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   if (t >= a.tokens) return;
@@ -404,49 +448,43 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(ExchangeRowsArg
     if (a.weights) weight = a.weights[t * a.k + lane];
     if (mine >= a.rows) mine = -1;
   }
-  const long long c0 = (long long)blockIdx.y * (32 * kPieces) + lane;
-  float acc[kPieces][N];
+  const long long c0 = (long long)blockIdx.y * (32 * P) + lane;
+  const V* in = static_cast<const V*>(a.in) + c0;
+  float acc[P][N];
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i)
+  for (int i = 0; i < P; ++i)
 #pragma unroll
     for (int n = 0; n < N; ++n) acc[i][n] = 0.f;
-  unsigned left = __ballot_sync(kFull, mine >= 0);
-  V next[kPieces];
-  auto fetch = [&](int j) {
-    const V* from = in + __shfl_sync(kFull, mine, j) * a.in_stride + c0;
+  for (unsigned left = __ballot_sync(kFull, mine >= 0); left; left &= left - 1) {
+    const int j = __ffs(left) - 1;
+    const V* from = in + __shfl_sync(kFull, mine, j) * a.in_stride;
+    const float w = __shfl_sync(kFull, weight, j);
+    V v[P];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i)
-      if (c0 + 32 * i < units) next[i] = from[32 * i];
-  };
-  if (left) fetch(__ffs(left) - 1);
-  while (left) {
-    const float w = __shfl_sync(kFull, weight, __ffs(left) - 1);
-    V v[kPieces];
+    for (int i = 0; i < P; ++i)
+      if (c0 + 32 * i < units) v[i] = load_row<STREAM>(from + 32 * i);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) v[i] = next[i];
-    left &= left - 1;
-    if (left) fetch(__ffs(left) - 1);
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i)
+    for (int i = 0; i < P; ++i)
 #pragma unroll
       for (int n = 0; n < N; ++n) acc[i][n] = fmaf(w, to_f(v[i].v[n]), acc[i][n]);
   }
   V* out = static_cast<V*>(a.out) + t * a.out_stride + c0;
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i)
+  for (int i = 0; i < P; ++i)
     if (c0 + 32 * i < units) {
-      V v;
+      V o;
 #pragma unroll
-      for (int n = 0; n < N; ++n) v.v[n] = from_f<T>(acc[i][n]);
-      out[32 * i] = v;
+      for (int n = 0; n < N; ++n) o.v[n] = from_f<T>(acc[i][n]);
+      out[32 * i] = o;
     }
 }
 
 // One CTA per token, its warps share the pieces: a piece of the gradient is read once and multiplied with and into
 // each of the token's rows.  The products of the pieces are added in a fixed order.
-template <typename T, int N>
+template <typename T, int N, bool STREAM>
 __global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(ExchangeRowsArgs a, long long units, unsigned token_blocks) {
   using V = Vec<T, N>;
+  constexpr int P = kPieces<sizeof(V)>;
   __shared__ float part[kRowWarps][kMaxChoices];
   V* out = static_cast<V*>(a.out);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -469,32 +507,25 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(Exchan
     if (mine >= a.rows) mine = -1;
   }
   const unsigned kept = __ballot_sync(kFull, mine >= 0);
-  for (long long c0 = (long long)warp * (32 * kPieces) + lane; c0 - lane < units; c0 += (long long)warps * (32 * kPieces)) {
+  for (long long c0 = (long long)warp * (32 * P) + lane; c0 - lane < units; c0 += (long long)warps * (32 * P)) {
     const V* from = static_cast<const V*>(a.in) + t * a.in_stride + c0;
-    V g[kPieces], next[kPieces];
+    const V* rows = static_cast<const V*>(a.saved) + c0;
+    V g[P];
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i)
+    for (int i = 0; i < P; ++i)
       if (c0 + 32 * i < units) g[i] = from[32 * i];
-    auto fetch = [&](int j) {
-      const V* row = static_cast<const V*>(a.saved) + __shfl_sync(kFull, mine, j) * a.saved_stride + c0;
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i)
-        if (c0 + 32 * i < units) next[i] = row[32 * i];
-    };
-    unsigned left = kept;
-    if (left) fetch(__ffs(left) - 1);
-    while (left) {
+    for (unsigned left = kept; left; left &= left - 1) {
       const int j = __ffs(left) - 1;
+      const long long r = __shfl_sync(kFull, mine, j);
       const float w = __shfl_sync(kFull, weight, j);
-      V* to = out + __shfl_sync(kFull, mine, j) * a.out_stride + c0;
-      V v[kPieces];
+      V v[P];
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) v[i] = next[i];
-      left &= left - 1;
-      if (left) fetch(__ffs(left) - 1);
+      for (int i = 0; i < P; ++i)
+        if (c0 + 32 * i < units) v[i] = load_row<STREAM>(rows + r * a.saved_stride + 32 * i);
+      V* to = out + r * a.out_stride + c0;
       float dot = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i)
+      for (int i = 0; i < P; ++i)
         if (c0 + 32 * i < units) {
           V o;
 #pragma unroll
@@ -503,7 +534,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(Exchan
             dot = fmaf(x, to_f(v[i].v[n]), dot);
             o.v[n] = from_f<T>(w * x);
           }
-          to[32 * i] = o;
+          store_row<STREAM>(to + 32 * i, o);
         }
       dot = warp_sum(dot);
       if (lane == j) dots += dot;
@@ -526,9 +557,11 @@ cudaError_t launch_route(const RouteArgs& a, cudaStream_t stream) { return route
 cudaError_t launch_route_backward(const RouteArgs& a, cudaStream_t stream) { return route_any<true>(a, stream); }
 
 cudaError_t launch_sort(const SortArgs& a, cudaStream_t stream) {
-  // warps first, then CTAs, each with a run of at least kSortRun assignments
+  // warps first, then CTAs, each with a run of at least kSortRun assignments; a warp scans at most 8 experts where
+  // the warps allow it
   const long long workers = (a.assignments + kSortRun - 1) / kSortRun;
-  const int warps = workers < 1 ? 1 : workers > kSortWarps ? kSortWarps : (int)workers;
+  const long long scanners = (a.experts + 7) / 8, both = workers > scanners ? workers : scanners;
+  const int warps = both > kSortWarps ? kSortWarps : (int)both;
   int ctas = 1;
   while (ctas < kSortCtas && (long long)ctas * kSortWarps < workers) ctas *= 2;
   const size_t bytes = sizeof(int) * ((size_t)warps * (a.experts | 1) + 4 * (size_t)a.experts);
@@ -571,41 +604,49 @@ int vector_bytes(const ExchangeRowsArgs& a) {
   return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : es;
 }
 
+bool streams(const ExchangeRowsArgs& a) { return a.rows * a.hidden * elem_size(a.dtype) > kStreamBytes; }
+
 // strides and lengths in vectors of `per` elements; the number of pieces of a row
-long long in_vectors(ExchangeRowsArgs& a, int per) {
+long long in_vectors(ExchangeRowsArgs& a, int per, int pieces) {
   a.hidden /= per;
   a.in_stride /= per;
   a.out_stride /= per;
   a.saved_stride /= per;
-  return (a.hidden + 32 * kPieces - 1) / (32 * kPieces);
+  return (a.hidden + 32 * pieces - 1) / (32 * pieces);
 }
 
 template <typename V>
 cudaError_t dispatch_as(ExchangeRowsArgs a, cudaStream_t stream) {
-  const long long pieces = in_vectors(a, (int)sizeof(V) / elem_size(a.dtype));
+  const bool streamed = streams(a);
+  const long long pieces = in_vectors(a, (int)sizeof(V) / elem_size(a.dtype), kPieces<sizeof(V)>);
   const unsigned token_blocks = (unsigned)((a.tokens + kRowWarps - 1) / kRowWarps);
   const unsigned clear_blocks = (unsigned)((a.rows + 32 * kRowWarps - 1) / (32 * kRowWarps));
   if (pieces > 65535) return cudaErrorInvalidConfiguration;
-  dispatch_kernel<V><<<dim3(token_blocks + clear_blocks, (unsigned)pieces), kRowWarps * 32, 0, stream>>>(a, a.hidden, token_blocks);
+  auto kernel = streamed ? dispatch_kernel<V, true> : dispatch_kernel<V, false>;
+  kernel<<<dim3(token_blocks + clear_blocks, (unsigned)pieces), kRowWarps * 32, 0, stream>>>(a, a.hidden, token_blocks);
   return cudaGetLastError();
 }
 
 template <typename T, int N>
 cudaError_t combine_as(ExchangeRowsArgs a, cudaStream_t stream) {
-  const long long pieces = in_vectors(a, N);
+  const bool streamed = streams(a);
+  const long long pieces = in_vectors(a, N, kPieces<sizeof(T) * N>);
   if (pieces > 65535) return cudaErrorInvalidConfiguration;
   const unsigned blocks = (unsigned)((a.tokens + kRowWarps - 1) / kRowWarps);
-  combine_kernel<T, N><<<dim3(blocks, (unsigned)pieces), kRowWarps * 32, 0, stream>>>(a, a.hidden);
+  auto kernel = streamed ? combine_kernel<T, N, true> : combine_kernel<T, N, false>;
+  kernel<<<dim3(blocks, (unsigned)pieces), kRowWarps * 32, 0, stream>>>(a, a.hidden);
   return cudaGetLastError();
 }
 
 template <typename T, int N>
 cudaError_t combine_backward_as(ExchangeRowsArgs a, cudaStream_t stream) {
-  const long long pieces = in_vectors(a, N);
+  const bool streamed = streams(a);
+  const long long pieces = in_vectors(a, N, kPieces<sizeof(T) * N>);
   const int warps = pieces < 1 ? 1 : pieces > kRowWarps ? kRowWarps : (int)pieces;
   const unsigned clear_blocks = (unsigned)((a.rows + 32 * warps - 1) / (32 * warps));
   if (a.tokens + clear_blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  combine_backward_kernel<T, N><<<(unsigned)a.tokens + clear_blocks, warps * 32, 0, stream>>>(a, a.hidden, (unsigned)a.tokens);
+  auto kernel = streamed ? combine_backward_kernel<T, N, true> : combine_backward_kernel<T, N, false>;
+  kernel<<<(unsigned)a.tokens + clear_blocks, warps * 32, 0, stream>>>(a, a.hidden, (unsigned)a.tokens);
   return cudaGetLastError();
 }
 
