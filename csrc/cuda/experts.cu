@@ -183,12 +183,14 @@ cudaError_t route_any(const RouteArgs& a, cudaStream_t stream) {
 //
 // One cluster of 1 to 16 CTAs; every warp owns a contiguous run of assignments.  Pass 1 counts each warp's
 // assignments per expert (the lanes that hold one expert find each other by a vote per bit of the expert's number
-// and elect a leader, so no count depends on the order of atomics), scans over the warps, over the CTAs (through distributed shared memory) and over the experts
-// turn the counts into each warp's first place per expert, pass 2 hands the places out in the order of the
-// assignments.  One launch and no workspace: what it costs is the latency of these steps, not its few bytes.
+// and elect a leader, so no count depends on the order of atomics) and leaves each assignment's place among them in
+// its slot.  Scans over the warps, over the CTAs (through distributed shared memory) and over the experts turn the
+// counts into first rows, which pass 2 adds.  One launch and no workspace: what it costs is the latency of these
+// steps and the votes of at most 512 warps, not its few bytes.
 constexpr int kSortWarps = 32;         // most warps of a CTA
 constexpr int kSortCtas = 16;          // most CTAs of the cluster
-constexpr int kSortRun = 128;          // assignments of a warp before another warp or CTA is added
+constexpr int kSortRun = 32;           // assignments of a warp before another warp or CTA is added (16384
+                                       // assignments take 11.0 us with runs of 128, 7.8 with 32)
 
 // The lanes that hold the same expert: a vote per bit.  (match_any does this in one instruction, but sorting 131072
 // assignments to 128 experts took 23.5 us with it and takes 17.9 with the votes.)
@@ -265,8 +267,12 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
     for (int j = 0; j < AHEAD; ++j) {
       if (base + 32 * j >= hi) break;
       const unsigned peers = same_expert(e[j], bits);
+      int place = 0;
+      if (e[j] >= 0) place = mine[e[j]] + __popc(peers & ((1u << lane) - 1));
+      __syncwarp();
       if (e[j] >= 0 && lane == __ffs(peers) - 1) mine[e[j]] += __popc(peers);
       __syncwarp();
+      if (base + 32 * j + lane < hi) a.slot[base + 32 * j + lane] = place;
     }
   }
   __syncthreads();
@@ -277,27 +283,29 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
     if (lane == 31) total[e] = x;
   }
   if (ctas > 1) { cluster_arrive(); cluster_wait(); } else __syncthreads();
-  for (int e = tid; e < E; e += threads) {
-    int sum = 0, earlier = 0;
-    if (ctas == 1) sum = total[e];
+  // one thread per expert: the launch has at least as many
+  int sum = 0, earlier = 0;
+  if (tid < E) {
+    if (ctas == 1) sum = total[tid];
     else
       for (int r = 0; r < ctas; ++r) {
-        const int c = remote_int(total + e, r);
+        const int c = remote_int(total + tid, r);
         if (r < rank) earlier += c;
         sum += c;
       }
-    before[e] = earlier;
-    all[e] = sum;
   }
   if (ctas > 1) cluster_arrive();       // this CTA has read the others' totals
+  const int upto = inclusive_scan(sum, lane);
+  __shared__ int warp_sum_of[kSortWarps];
+  if (lane == 31) warp_sum_of[warp] = upto;
   __syncthreads();
-  if (warp == 0) {                      // exclusive scan over the experts
-    int carry = 0;
-    for (int base = 0; base < E; base += 32) {
-      const int e = base + lane, c = e < E ? all[e] : 0, x = inclusive_scan(c, lane);
-      if (e < E) first[e] = carry + x - c;
-      carry += __shfl_sync(kFull, x, 31);
-    }
+  int start = upto - sum;
+  for (int w = 0; w < warp; ++w) start += warp_sum_of[w];
+  if (tid < E) {
+    all[tid] = sum;
+    first[tid] = start;
+    // pass 2 adds one number: the first row of this CTA's assignments, or their first place under a capacity
+    before[tid] = a.capacity ? earlier : start + earlier;
   }
   __syncthreads();
   if (rank == 0)
@@ -314,29 +322,24 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
       a.source[r] = -1;
   }
   for (long long base = lo; base < hi; base += 32 * AHEAD) {
-    int e[AHEAD];
-#pragma unroll
-    for (int j = 0; j < AHEAD; ++j) e[j] = expert_of<I>(a, base + 32 * j + lane, hi);
+    int e[AHEAD], place[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
       const long long i = base + 32 * j + lane;
-      if (base + 32 * j >= hi) break;
-      const unsigned peers = same_expert(e[j], bits);
-      int place = 0;
-      if (e[j] >= 0) place = mine[e[j]] + __popc(peers & ((1u << lane) - 1));
-      __syncwarp();
-      if (e[j] >= 0 && lane == __ffs(peers) - 1) mine[e[j]] += __popc(peers);
-      __syncwarp();
-      if (i < hi) {
-        int row = -1;
-        if (e[j] >= 0) {
-          place += before[e[j]];
-          if (a.capacity == 0) row = first[e[j]] + place;
-          else if (place < a.capacity) row = (int)(e[j] * a.capacity + place);
-        }
-        a.slot[i] = row;
-        if (row >= 0) a.source[row] = (int)i;
+      e[j] = expert_of<I>(a, i, hi);
+      place[j] = i < hi ? a.slot[i] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const long long i = base + 32 * j + lane;
+      if (i >= hi) continue;
+      int row = -1;
+      if (e[j] >= 0) {
+        place[j] += mine[e[j]] + before[e[j]];
+        row = a.capacity == 0 ? place[j] : place[j] < a.capacity ? (int)(e[j] * a.capacity + place[j]) : -1;
       }
+      a.slot[i] = row;
+      if (row >= 0) a.source[row] = (int)i;
     }
   }
   if (ctas > 1) cluster_wait();         // the totals stay until every CTA has read them
