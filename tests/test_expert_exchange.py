@@ -1,0 +1,195 @@
+"""Expert-parallel token exchange: one rank through the engine, two ranks as threads that exchange host-side."""
+import threading
+from types import SimpleNamespace
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from vericcl_b200.errors import RuntimeFailure                    # noqa: E402
+from vericcl_b200.models import ExpertExchange                    # noqa: E402
+from vericcl_b200.ops import experts as ex                        # noqa: E402
+
+
+def test_refusals():
+    engine = SimpleNamespace(comm=SimpleNamespace(world=2))
+    good = dict(experts=4, hidden=8, capacity=2, dtype=torch.bfloat16)
+    for change in (dict(experts=3), dict(experts=0), dict(experts=2048), dict(hidden=0), dict(capacity=0),
+                   dict(capacity=1 << 30), dict(dtype=torch.float64), dict(hidden=3, capacity=1)):
+        with pytest.raises(RuntimeFailure):
+            ExpertExchange(engine, **{**good, **change})
+
+
+def gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+
+
+def tokens_for(rank, tokens, experts, k, hidden, dtype):
+    g = torch.Generator(device="cuda").manual_seed(100 + rank)
+    x = torch.randn(tokens, hidden, device="cuda", generator=g).to(dtype)
+    logits = torch.randn(tokens, experts, device="cuda", generator=g)
+    grad = torch.randn(tokens, hidden, device="cuda", generator=g).to(dtype)
+    return x, logits, grad
+
+
+def layer(exchange, x, logits, grad, k, scale):
+    """A mixture whose expert e multiplies its rows with scale[e]; forward and backward."""
+    ids, w = ex.route(logits, k)
+    rows = exchange.dispatch(x, ids)
+    per_row = scale.repeat_interleave(exchange.capacity).repeat(exchange.comm.world)[:, None].to(x.dtype)
+    out = exchange.combine(rows * per_row, w)
+    grad_rows, grad_w = exchange.combine_backward(grad, w)
+    grad_x = exchange.dispatch_backward(grad_rows * per_row)
+    return [t.clone() for t in (out, grad_x, grad_w, ids, exchange.counts, exchange.order.slot)]
+
+
+def plain_layer(x, logits, grad, k, scale, capacity):
+    """The same on one rank's tokens without any exchange, in 64 bits; powers of two as scales keep rows exact."""
+    ids, w = ex.route(logits, k)
+    order = ex.sort_by_expert(ids, scale.numel(), capacity=capacity)
+    kept = (order.slot >= 0).double()
+    factor = scale.double()[ids.long()] * kept
+    out = (x.double()[:, None] * (factor * w.double())[..., None]).sum(1)
+    grad_x = (grad.double()[:, None] * (factor * w.double())[..., None]).sum(1)
+    grad_w = (grad.double()[:, None] * x.double()[:, None] * factor[..., None]).sum(2)
+    return out, grad_x, grad_w
+
+
+def compare(got, want, x, grad, scale, dtype):
+    half = torch.finfo(dtype).eps / 2
+    k, hidden, top = got[3].size(1), x.size(1), scale.abs().max().item()
+    fp32 = (2 * k + 2) * 2.0 ** -24
+    # out: one rounding of sums of at most k products of magnitude |x| top (weights sum to at most 1)
+    assert bool(((got[0].double() - want[0]).abs() <= half * want[0].abs() + fp32 * x.abs().max().double() * top).all())
+    # grad_x: w * grad is rounded once per row before the k rows are added, then once more
+    bound = (half * 2.01 + fp32) * grad.abs().max().double() * top
+    assert bool(((got[1].double() - want[1]).abs() <= bound).all())
+    size = (grad.double().abs() * x.double().abs()).sum(1, keepdim=True) * top
+    assert bool(((got[2].double() - want[2]).abs() <= (hidden + 1) * 2.0 ** -24 * size).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_one_rank(dtype):
+    gpu()
+    from vericcl_b200.models import CollectiveEngine
+    from vericcl_b200.parallel import Communicator
+    comm = Communicator(heap_bytes=64 << 20)
+    try:
+        exchange = ExpertExchange(CollectiveEngine(comm), experts=6, hidden=72, capacity=9, dtype=dtype)
+        with pytest.raises(RuntimeFailure, match="first"):
+            exchange.combine(torch.zeros(54, 72, dtype=dtype, device="cuda"), torch.zeros(1, 1, device="cuda"))
+        scale = torch.tensor([1.0, 2, 0.5, -1, 4, -0.25], device="cuda")
+        for tokens in (25, 1, 0):
+            x, logits, grad = tokens_for(0, tokens, 6, 2, 72, dtype)
+            if tokens:
+                compare(layer(exchange, x, logits, grad, 2, scale), plain_layer(x, logits, grad, 2, scale, 9), x, grad,
+                        scale, dtype)
+            else:
+                rows = exchange.dispatch(x, torch.zeros(0, 2, dtype=torch.int32, device="cuda"))
+                assert bool((rows == 0).all()) and int(exchange.counts.sum()) == 0
+        with pytest.raises(RuntimeFailure):
+            exchange.dispatch(x[:, :8], torch.zeros(0, 2, dtype=torch.int32, device="cuda"))
+        used = comm.heap.used()
+        exchange.close()
+        assert comm.heap.used() < used
+    finally:
+        comm.close()
+
+
+class Threads:
+    """Two ranks' AllToAll as copies between two barriers: nothing on the GPU waits."""
+
+    def __init__(self, world):
+        self.world, self.gate, self.parts = world, threading.Barrier(world, timeout=60), {}
+
+    def engine(self, rank):
+        comm = SimpleNamespace(world=self.world, rank=rank, free=lambda t: None,
+                               empty=lambda n, dtype=torch.float32: torch.empty(n, dtype=dtype, device="cuda"))
+
+        def all_to_all(inp, out):
+            torch.cuda.synchronize()
+            self.parts[rank] = inp.reshape(self.world, -1)
+            self.gate.wait()
+            for r in range(self.world):
+                out.view(self.world, -1)[r].copy_(self.parts[r][rank])
+            torch.cuda.synchronize()
+            self.gate.wait()
+        return SimpleNamespace(comm=comm, all_to_all=all_to_all)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_two_ranks(dtype):
+    gpu()
+    world, experts, k, hidden, capacity = 2, 6, 2, 64, 5
+    scale = torch.tensor([1.0, 2, 0.5, -1, 4, -0.25], device="cuda")
+    links, results, errors = Threads(world), {}, []
+
+    def rank_main(rank):
+        try:
+            exchange = ExpertExchange(links.engine(rank), experts=experts, hidden=hidden, capacity=capacity, dtype=dtype)
+            x, logits, grad = tokens_for(rank, 17 + rank, experts, k, hidden, dtype)
+            local = scale[rank * 3:rank * 3 + 3]
+            results[rank] = layer(exchange, x, logits, grad, k, local)
+        except Exception as error:                               # noqa: BLE001  (reported by the test)
+            errors.append(error)
+            links.gate.abort()
+
+    threads = [threading.Thread(target=rank_main, args=(r,)) for r in range(world)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for rank in range(world):
+        x, logits, grad = tokens_for(rank, 17 + rank, experts, k, hidden, dtype)
+        compare(results[rank], plain_layer(x, logits, grad, k, scale, capacity), x, grad, scale, dtype)
+        # the counts a rank holds are those of its experts, by source rank
+        want = []
+        for source in range(world):
+            slot = results[source][5]
+            ids = results[source][3]
+            want += [int(((ids == e) & (slot >= 0)).sum()) for e in range(rank * 3, rank * 3 + 3)]
+        assert results[rank][4].tolist() == want
+
+
+@pytest.mark.gpu
+def test_int4_products_of_exchanged_rows():
+    gpu()
+    world, experts, hidden, capacity = 2, 4, 64, 3
+    links, results, errors = Threads(world), {}, []
+    g = torch.Generator(device="cuda").manual_seed(7)
+    packed, scales = ex.quantize_int4(torch.randn(experts, hidden, hidden, device="cuda", generator=g).bfloat16(), 32)
+
+    def rank_main(rank):
+        try:
+            exchange = ExpertExchange(links.engine(rank), experts=experts, hidden=hidden, capacity=capacity)
+            x, logits, _ = tokens_for(rank, 4, experts, 1, hidden, torch.bfloat16)
+            ids, w = ex.route(logits, 1)
+            mine = slice(rank * 2, rank * 2 + 2)
+            rows = exchange.dispatch(x, ids)
+            out = exchange.combine(exchange.matmul_int4(rows, packed[mine].contiguous(), scales[mine].contiguous()), w)
+            with pytest.raises(RuntimeFailure):
+                exchange.matmul_int4(rows, packed, scales)
+            results[rank] = (out.clone(), ids.clone(), exchange.order.slot.clone(), x)
+        except Exception as error:                               # noqa: BLE001  (reported by the test)
+            errors.append(error)
+            links.gate.abort()
+
+    threads = [threading.Thread(target=rank_main, args=(r,)) for r in range(world)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    q = torch.stack([packed & 15, packed >> 4], -1).flatten(-2).double() - 8
+    dense = (q.unflatten(-1, (-1, 32)) * scales.double()[..., None]).flatten(-2)
+    for out, ids, slot, x in results.values():
+        for t in range(4):
+            want = dense[ids[t, 0]] @ x[t].double() if slot[t, 0] >= 0 else torch.zeros(hidden, dtype=torch.float64,
+                                                                                       device="cuda")
+            # one weight (1.0), one rounding of the product; fp32 sums of 64 terms
+            size = dense[ids[t, 0]].abs() @ x[t].double().abs()
+            assert bool(((out[t].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * size).all())
