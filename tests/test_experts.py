@@ -631,3 +631,16 @@ def test_out_over_an_input_is_refused():
         ex.dispatch(x[:4], order, out=x[2:6])
     with pytest.raises(RuntimeFailure, match="overlaps"):
         ex.combine(x[:4], torch.zeros(4, 1, device="cuda"), order, out=x[:4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kernel", ["expert_route", "expert_sort", "expert_dispatch", "expert_combine",
+                                    "expert_combine_backward", "expert_matmul_int4"])
+def test_kernel_bench_runs_the_expert_kernels(kernel, capsys):
+    cuda()
+    import json
+    from vericcl_b200.ops import kernel_bench
+    assert kernel_bench.main(["--kernel", kernel, "--tokens", "33", "--experts", "8", "--choices", "2", "--hidden", "256",
+                              "--outputs", "48", "--group", "64", "--iters", "2"]) == 0
+    line = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
+    assert line["us"] > 0 and kernel in line["kernel"]

@@ -3,10 +3,16 @@
     python -m vericcl_b200.ops.kernel_bench --kernel local_reduce --k 4 --elems 67108864 --dtype bfloat16
     python -m vericcl_b200.ops.kernel_bench --kernel fp8_allgather --elems 268435456 --dtype bfloat16
     python -m vericcl_b200.ops.kernel_bench --kernel push_allgather --elems 268435456 --dtype bfloat16
+    python -m vericcl_b200.ops.kernel_bench --kernel expert_dispatch --tokens 16384 --experts 128 --choices 8 --hidden 4096
+    python -m vericcl_b200.ops.kernel_bench --kernel expert_matmul_int4 --tokens 32 --experts 32 --choices 8 --hidden 4096 --outputs 2048
 
 Options: ``--k`` sources of the local reduce, ``--no-scale`` (K = 1 is then a plain
 copy), ``--lean`` (the register-lean instance), ``--bulk 1|3`` (TMA-staged loads,
 and TMA stores for plain copies), ``--fanout`` (push AllGather fan-out order).
+The expert kernels (``expert_route``, ``expert_sort``, ``expert_dispatch``,
+``expert_combine``, ``expert_combine_backward``, ``expert_matmul_int4``) take
+``--tokens --experts --choices --hidden`` and, for the 4-bit products,
+``--outputs --group``; their tokens choose experts at random.
 
 Each run: ``--warmup`` untimed launches, then ``--iters`` launches between two
 CUDA events on the current stream; the inputs are larger than the 126 MB L2
@@ -35,9 +41,46 @@ def hbm_peak_gbs() -> tuple:
         return 6650.0, "fallback"
 
 
+EXPERT_KERNELS = ("expert_route", "expert_sort", "expert_dispatch", "expert_combine", "expert_combine_backward",
+                  "expert_matmul_int4")
+
+
+def expert_case(args, dtype):
+    """``(call, algorithmic bytes, label)`` of one expert kernel on random choices."""
+    from vericcl_b200.ops import experts as ops
+    t, e, k, h = args.tokens, args.experts, args.choices, args.hidden
+    esize, rows = dtype.itemsize, t * k
+    logits = torch.randn(t, e, device="cuda").to(dtype)
+    ids, weights = ops.route(logits, k)
+    order = ops.sort_by_expert(ids, e)
+    label = "%s T=%d E=%d k=%d" % (args.kernel, t, e, k)
+    if args.kernel == "expert_route":
+        return lambda: ops.route(logits, k), t * e * esize + 8 * rows, label
+    if args.kernel == "expert_sort":
+        return lambda: ops.sort_by_expert(ids, e), 12 * rows + 8 * e, label
+    x = torch.randn(t, h, device="cuda").to(dtype)
+    label += " H=%d" % h
+    if args.kernel == "expert_dispatch":
+        out = torch.empty(rows, h, device="cuda", dtype=dtype)
+        return lambda: ops.dispatch(x, order, out=out), (t + rows) * h * esize + 8 * rows, label
+    values = torch.randn(rows, h, device="cuda").to(dtype)
+    if args.kernel == "expert_combine":
+        return lambda: ops.combine(values, weights, order), (t + rows) * h * esize + 8 * rows, label
+    if args.kernel == "expert_combine_backward":
+        out = torch.empty_like(values)
+        return (lambda: ops.combine_backward(x, values, weights, order, out=out),
+                (t + 2 * rows) * h * esize + 16 * rows, label)
+    packed = torch.randint(0, 256, (e, args.outputs, h // 2), dtype=torch.uint8, device="cuda")
+    scales = torch.rand(e, args.outputs, h // args.group, device="cuda").to(dtype)
+    used = int((order.counts > 0).sum())
+    return (lambda: ops.expert_matmul_int4(values, order.starts, order.counts, packed, scales),
+            used * args.outputs * (h // 2 + h // args.group * esize) + rows * (h + args.outputs) * esize,
+            label + " N=%d group %d, %d experts used" % (args.outputs, args.group, used))
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="vericcl_b200.ops.kernel_bench")
-    ap.add_argument("--kernel", required=True, choices=("local_reduce", "fp8_allgather", "push_allgather"))
+    ap.add_argument("--kernel", required=True, choices=("local_reduce", "fp8_allgather", "push_allgather") + EXPERT_KERNELS)
     ap.add_argument("--elems", type=int, default=64 << 20)
     ap.add_argument("--k", type=int, default=4, help="sources of the local reduce")
     ap.add_argument("--dtype", default="bfloat16", choices=sorted(DTYPES))
@@ -47,6 +90,12 @@ def main(argv=None) -> int:
     ap.add_argument("--no-scale", action="store_true", help="local reduce: no scale (K=1 is then a plain copy)")
     ap.add_argument("--lean", action="store_true", help="local reduce: the register-lean instance (one-rank default)")
     ap.add_argument("--fanout", action="store_true", help="push AllGather: the fan-out mode")
+    ap.add_argument("--tokens", type=int, default=16384, help="expert kernels: tokens")
+    ap.add_argument("--experts", type=int, default=128, help="expert kernels: experts")
+    ap.add_argument("--choices", type=int, default=8, help="expert kernels: choices per token")
+    ap.add_argument("--hidden", type=int, default=4096, help="expert kernels: columns of a token")
+    ap.add_argument("--outputs", type=int, default=2048, help="4-bit products: outputs per expert")
+    ap.add_argument("--group", type=int, default=128, choices=(32, 64, 128), help="4-bit products: values per scale")
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--iters", type=int, default=10)
     args = ap.parse_args(argv)
@@ -54,12 +103,14 @@ def main(argv=None) -> int:
     from vericcl_b200.parallel import Communicator
     dtype = DTYPES[args.dtype]
     esize = torch.tensor([], dtype=dtype).element_size()
-    n = args.elems
+    n = 0 if args.kernel in EXPERT_KERNELS else args.elems
     heap = 3 * n * esize + (256 << 20)
     comm = Communicator(heap_bytes=heap)
     mod = comm._mod
     stream = torch.cuda.current_stream()
-    if args.kernel == "local_reduce":
+    if args.kernel in EXPERT_KERNELS:
+        fn, nbytes, label = expert_case(args, dtype)
+    elif args.kernel == "local_reduce":
         srcs = torch.randn(args.k, n, device="cuda").to(dtype)
         dst = torch.empty(n, device="cuda", dtype=dtype)
         lanes = args.lanes or min(148, mod.max_ctas(512))
