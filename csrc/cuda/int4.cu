@@ -36,7 +36,7 @@ constexpr int kBoxes = 2;             // boxes of a tile
 constexpr int kTileK = kBoxes * kBoxK;
 constexpr int kStages = 2;            // tiles in flight of a warp
 constexpr unsigned kBoxBytes = 16 * 128;
-constexpr int kStage = 16 * 1024;      // inner values x rows of x staged at a time: 32 KB
+constexpr int kPool = 44 * 1024;      // shared memory for a stage of x and scales
 constexpr unsigned kTileBytes = kBoxes * kBoxBytes;
 constexpr unsigned kFull = 0xffffffffu;
 
@@ -145,14 +145,34 @@ __device__ __forceinline__ float remote_f(unsigned addr, unsigned rank) {
   return v;
 }
 
-// PAIR groups of 16 weight rows times COLS x 8 rows of x, scaled and added to acc.  `x` is the lane's first unit.
-// The groups' products alternate, and with one column each group's sum is kept in two halves, so that a product
+// scales of PAIR groups of one weight row
+template <int PAIR>
+__device__ __forceinline__ void load_scales(float (&f)[PAIR], const float* s) {
+#pragma unroll
+  for (int p = 0; p < PAIR; ++p) f[p] = s[p];
+}
+template <int PAIR, typename S>
+__device__ __forceinline__ void load_scales(float (&f)[PAIR], const S* s) {
+  if constexpr (PAIR == 2) {                // at an even place: one word
+    const unsigned w = *reinterpret_cast<const unsigned*>(s);
+    const unsigned short lo = (unsigned short)w, hi = (unsigned short)(w >> 16);
+    f[0] = to_f(*reinterpret_cast<const S*>(&lo));
+    f[1] = to_f(*reinterpret_cast<const S*>(&hi));
+  } else {
+    f[0] = to_f(s[0]);
+  }
+}
+
+// PAIR groups of 16 weight rows times COLS x 8 rows of x, scaled and added to acc.  `x` is the lane's first unit, the
+// next word's is `step` units further (32 * COLS, or with one column 4 times its rows rounded to a power of two);
+// `scale` points to the lane's first weight row, the second is `second` further.
+// The groups' products alternate, and with one column and longer groups each group's sum is kept in two halves, so that a product
 // seldom waits for the one before it.  A lane whose row of x does not exist computes with what lies there: columns
 // of a product do not mix, and that column is not written.
 template <typename T, typename S, int VEC, int COLS, int PAIR>
 __device__ __forceinline__ void group_product(float (&acc)[COLS][4], const unsigned char* tile, unsigned at, int u0,
-                                              const uint4* x, const S* scale) {
-  constexpr int HALVES = COLS == 1 ? 2 : 1;
+                                              const uint4* x, int step, const S* scale, int second) {
+  constexpr int HALVES = COLS == 1 && VEC > 1 ? 2 : 1;
   unsigned ra[PAIR][VEC], rb[PAIR][VEC];
   float part[PAIR][HALVES][COLS][4];
 #pragma unroll
@@ -172,14 +192,17 @@ __device__ __forceinline__ void group_product(float (&acc)[COLS][4], const unsig
       const unsigned vb[4] = {two_values<T, 0>(wb), two_values<T, 1>(wb), two_values<T, 0>(wb >> 8), two_values<T, 1>(wb >> 8)};
 #pragma unroll
       for (int t = 0; t < COLS; ++t) {
-        const uint4 b = x[((p * VEC + v) * COLS + t) * 32];
+        const uint4 b = x[(p * VEC + v) * (COLS == 1 ? step : 32 * COLS) + t * 32];
         mma<T>(part[p][0][t], va, vb, 0, b.x, b.y, v == 0);
         mma<T>(part[p][HALVES - 1][t], va, vb, 2, b.z, b.w, HALVES == 2 && v == 0);
       }
     }
+  float first[PAIR], other[PAIR];
+  load_scales<PAIR>(first, scale);
+  load_scales<PAIR>(other, scale + second);
 #pragma unroll
   for (int p = 0; p < PAIR; ++p) {
-    const float sa = to_f(scale[p * kTileN]), sb = to_f(scale[p * kTileN + 8]);
+    const float sa = first[p], sb = other[p];
 #pragma unroll
     for (int t = 0; t < COLS; ++t)
 #pragma unroll
@@ -197,6 +220,9 @@ struct Geometry {
   unsigned n_tiles, items;
 };
 
+// rows of a unit of x with one column: a power of two
+__device__ __forceinline__ int staged_rows(int rows) { return rows > 4 ? 8 : rows > 2 ? 4 : rows; }
+
 struct Item {
   int expert, row0, rows;    // rows of x: row0 ... row0 + rows - 1, at most 32
   long long n0;              // the CTA's first weight row
@@ -209,7 +235,6 @@ template <typename T, typename S, int VEC, int COLS>
 __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args& a, const Geometry& geo, const Item& it,
                                           unsigned char* smem, unsigned bars) {
   constexpr int GROUP = 32 * VEC, UNITS = kTileK / GROUP;               // groups of a tile
-  constexpr int CHUNK = kStage / (8 * COLS) / kTileK * UNITS;           // groups of a stage, whole tiles
   constexpr int PAIR = COLS <= 2 ? 2 : 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tq = lane & 3;
   const int groups = (int)(a.inner / GROUP), units = (it.k_hi - it.k_lo) / GROUP, tiles = (units + UNITS - 1) / UNITS;
@@ -227,10 +252,15 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
   const int row = VEC == 4 ? (g & 1) * 4 + (g >> 1) : VEC == 2 ? (g & 3) * 2 + (g >> 2) : g;
   const unsigned lane_at = row * 128 + (((tq * VEC / 4) ^ row) << 4) + (tq * VEC % 4) * 4;
   const T* x = static_cast<const T*>(a.x) + it.row0 * a.x_stride + it.k_lo;
-  const S* scales = static_cast<const S*>(a.scales) + (base + min(it.n0 + (tid & (kTileN - 1)), a.n - 1)) * groups + it.k_lo / GROUP;
+  const S* scales = static_cast<const S*>(a.scales) + it.k_lo / GROUP;
   unsigned char* staged = smem + (kThreads / 32) * kStages * kTileBytes;
-  uint4* xs = reinterpret_cast<uint4*>(staged);                         // [groups * VEC][8 * COLS][4]
-  S* sc = reinterpret_cast<S*>(staged + kStage * 2);                    // [groups][kTileN]
+  // a stage takes as many tiles as the pool holds, equal numbers in all stages; fewer rows of x leave room for more
+  const int unit = COLS == 1 ? staged_rows(it.rows) : 8 * COLS, step = 4 * unit;
+  const int fits = kPool / (kTileK * 2 * unit + kTileN * (UNITS * (int)sizeof(S) + 8)), stages = (tiles + fits - 1) / fits;
+  const int chunk = (tiles + stages - 1) / max(stages, 1) * UNITS;      // groups
+  const int pitch = sizeof(S) == 4 ? chunk | 1 : 2 * ((chunk + 1) / 2 | 1);   // an odd number of words: no bank conflicts
+  uint4* xs = reinterpret_cast<uint4*>(staged);                         // [groups * VEC][unit][4]
+  S* sc = reinterpret_cast<S*>(staged + chunk * GROUP * 2 * unit);      // [kTileN][pitch]
   float acc[COLS][4];
 #pragma unroll
   for (int t = 0; t < COLS; ++t)
@@ -240,11 +270,22 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
   unsigned phase = 0;
   int late = -1;                            // the tile that did not come
 
-  for (int c0 = 0; c0 < units; c0 += CHUNK) {
-    const int here = min(CHUNK, units - c0), eighths = here * (GROUP / 8);
+  for (int c0 = 0; c0 < units; c0 += chunk) {
+    const int here = min(chunk, units - c0), eighths = here * (GROUP / 8);
     if (c0) __syncthreads();                // the stage before has been read
-    // x as 16-byte units of 8 inner values in the order 0 4 1 5 2 6 3 7; four loads are in flight per thread
+    // a warp stages the scales of its own rows, along the groups (of two rows at once where those are few), and its
+    // share of x: 16-byte units of 8 inner values in the order 0 4 1 5 2 6 3 7, four loads in flight
     {
+      const bool narrow = here <= 16;
+      const int su = narrow ? lane & 15 : lane, sr = narrow ? lane >> 4 : 0, rows_at_once = narrow ? 2 : 1;
+      S sv[8];
+      auto ask = [&](int r0, int u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (u < here)
+            sv[i] = scales[(base + min(it.n0 + warp * 16 + r0 + i * rows_at_once + sr, a.n - 1)) * groups + c0 + u];
+      };
+      ask(0, su);                           // on its way while x is staged
       const T* p = x + (long long)c0 * GROUP;
       int token = tid / eighths, k8 = tid - token * eighths;
       while (token < it.rows) {
@@ -264,7 +305,7 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
               v[i] = *reinterpret_cast<uint4*>(e);
             }
             const int grp = k8 / (4 * VEC), in = k8 % (4 * VEC);        // in = (lane % 4) * VEC + word
-            at[i] = ((grp * VEC + in % VEC) * (8 * COLS) + token) * 4 + in / VEC;
+            at[i] = ((grp * VEC + in % VEC) * unit + token) * 4 + in / VEC;
           }
           k8 += kThreads;
           while (k8 >= eighths) { k8 -= eighths; ++token; }
@@ -275,19 +316,19 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
             xs[at[i]] = make_uint4(__byte_perm(v[i].x, v[i].z, 0x5410), __byte_perm(v[i].x, v[i].z, 0x7632),
                                    __byte_perm(v[i].y, v[i].w, 0x5410), __byte_perm(v[i].y, v[i].w, 0x7632));
       }
-    }
-    for (int u0 = tid / kTileN; u0 < here; u0 += 8 * (kThreads / kTileN)) {
-      S v[8];
+      for (int r0 = 0, u = su;;) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (u0 + i * (kThreads / kTileN) < here) v[i] = scales[c0 + u0 + i * (kThreads / kTileN)];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (u0 + i * (kThreads / kTileN) < here) sc[(u0 + i * (kThreads / kTileN)) * kTileN + (tid & (kTileN - 1))] = v[i];
+        for (int i = 0; i < 8; ++i)
+          if (u < here) sc[(warp * 16 + r0 + i * rows_at_once + sr) * pitch + u] = sv[i];
+        u += 32;
+        if (u - su >= here) { u = su; r0 += 8 * rows_at_once; }
+        if (r0 == 16) break;
+        ask(r0, u);
+      }
     }
     __syncthreads();
     const uint4* xw = xs + g * 4 + tq;
-    const S* sw = sc + warp * 16 + row;
+    const S* sw = sc + (warp * 16 + row) * pitch;
     if (busy)
       for (int u0 = 0; u0 < here; u0 += UNITS) {
         if (late < 0 && !__all_sync(kFull, wait_tile(bar + 8 * slot, phase))) late = (c0 + u0) / UNITS;
@@ -295,13 +336,13 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
         if (u0 + UNITS <= here) {
 #pragma unroll
           for (int u = 0; u < UNITS; u += PAIR)
-            group_product<T, S, VEC, COLS, PAIR>(acc, tile, lane_at, u, xw + u * VEC * COLS * 32, sw + u * kTileN);
+            group_product<T, S, VEC, COLS, PAIR>(acc, tile, lane_at, u, xw + u * VEC * step, step, sw + u, 8 * pitch);
         } else {
           for (int u = 0; u0 + u < here; ++u)
-            group_product<T, S, VEC, COLS, 1>(acc, tile, lane_at, u, xw + u * VEC * COLS * 32, sw + u * kTileN);
+            group_product<T, S, VEC, COLS, 1>(acc, tile, lane_at, u, xw + u * VEC * step, step, sw + u, 8 * pitch);
         }
-        xw += UNITS * VEC * COLS * 32;
-        sw += UNITS * kTileN;
+        xw += UNITS * VEC * step;
+        sw += UNITS;
         __syncwarp();                       // the tile has been read by every lane
         const int coming = (c0 + u0) / UNITS + kStages;
         if (lane == 0 && coming < tiles && late < 0)
@@ -437,7 +478,6 @@ __global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_
 
 template <typename T, typename S, int VEC>
 cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
-  constexpr int GROUP = 32 * VEC;
   // items: every segment's last may be partial
   const long long items = (a.rows + kItem - 1) / kItem + (a.segments < a.rows ? a.segments : a.rows) - 1;
   const long long n_tiles = (a.n + kTileN - 1) / kTileN;
@@ -450,9 +490,7 @@ cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
   geo.n_tiles = (unsigned)n_tiles;
   geo.items = (unsigned)items;
   geo.aligned = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_stride % 8 == 0;
-  size_t bytes = (size_t)kStage * 2 + (size_t)kStage / 8 / GROUP * kTileN * sizeof(S);
-  const size_t sums = sizeof(float) * kItem * kTileN;
-  if (bytes < sums) bytes = sums;
+  size_t bytes = kPool;
   bytes += kThreads / 32 * kStages * kTileBytes + 1024;
   CUtensorMap map;
   const cuuint64_t size[2] = {(cuuint64_t)(a.inner / 2), (cuuint64_t)a.experts * a.n}, pitch[1] = {(cuuint64_t)(a.inner / 2)};
