@@ -286,15 +286,18 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
             sv[i] = scales[(base + min(it.n0 + warp * 16 + r0 + i * rows_at_once + sr, a.n - 1)) * groups + c0 + u];
       };
       ask(0, su);                           // on its way while x is staged
+      // a row's units go to 8 / unit warps (one where there are 8 rows or more)
+      const int at_once = COLS == 1 ? unit : 8, parts = 8 / at_once;
+      const int k8_first = (warp / at_once) * 32 + lane, k8_step = 32 * parts;
       const T* p = x + (long long)c0 * GROUP;
-      int token = tid / eighths, k8 = tid - token * eighths;
+      int token = warp % at_once, k8 = k8_first;
       while (token < it.rows) {
         uint4 v[4];
         int at[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           at[i] = -1;
-          if (token < it.rows) {
+          if (token < it.rows && k8 < eighths) {
             const T* from = p + token * a.x_stride + 8 * k8;
             if (geo.aligned) {
               v[i] = *reinterpret_cast<const uint4*>(from);
@@ -307,8 +310,8 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
             const int grp = k8 / (4 * VEC), in = k8 % (4 * VEC);        // in = (lane % 4) * VEC + word
             at[i] = ((grp * VEC + in % VEC) * unit + token) * 4 + in / VEC;
           }
-          k8 += kThreads;
-          while (k8 >= eighths) { k8 -= eighths; ++token; }
+          k8 += k8_step;
+          if (k8 - lane >= eighths) { k8 = k8_first; token += at_once; }
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -368,7 +371,8 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
   }
 }
 
-template <typename T, typename S, int VEC>
+// MOST: the most columns of 8 rows of x an item of this call can have.
+template <typename T, typename S, int VEC, int MOST>
 __global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_constant__ CUtensorMap map, Int4Args a,
                                                                 Geometry geo) {
   extern __shared__ unsigned char dynamic[];
@@ -376,17 +380,19 @@ __global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_
   unsigned char* smem = dynamic + (-(unsigned)__cvta_generic_to_shared(dynamic) & 1023u);
   __shared__ __align__(8) unsigned long long bars[kThreads / 32][kStages];
   __shared__ int pick[3];                   // segment, first row, rows of this CTA's item
-  __shared__ int2 scan[kThreads / 32];
+  __shared__ int3 scan[kThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned rank = cluster_rank(), ranks = cluster_size();
   const int item = (int)(blockIdx.x / ranks / geo.n_tiles);
   const long long n0 = (long long)(blockIdx.x / ranks % geo.n_tiles) * kTileN;
 
-  // which segment and rows: the items count the segments' tiles of kItem rows
+  // which segment and rows: the items are the segments' tiles of kItem rows, those of more than 8 rows first, so that
+  // the longer ones do not start last
   int covered = 0;                          // rows that some segment covers
   {
     constexpr int PER = 1024 / kThreads;    // at most 1024 segments, PER consecutive ones a thread
-    int first[PER], count[PER], mine = 0, rows = 0;
+    int first[PER], count[PER], rows = 0;
+    int2 mine = make_int2(0, 0);            // longer and shorter items
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int s = tid * PER + i;
@@ -398,38 +404,44 @@ __global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_
       const long long lo = first[i], hi = min(lo + count[i], a.rows);
       first[i] = max(first[i], 0);
       count[i] = (int)max(hi - first[i], 0ll);
-      mine += (count[i] + kItem - 1) / kItem;
+      mine.x += (count[i] + kItem - 9) / kItem;
+      mine.y += (unsigned)(count[i] - 1) % kItem < 8 && count[i];
       rows += count[i];
     }
-    int x = mine;
+    int2 x = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const int y = __shfl_up_sync(kFull, x, off);
-      if (lane >= off) x += y;
+      const int y = __shfl_up_sync(kFull, x.x, off), z = __shfl_up_sync(kFull, x.y, off);
+      if (lane >= off) x.x += y, x.y += z;
     }
     rows = __reduce_add_sync(kFull, rows);
-    if (lane == 31) scan[warp] = make_int2(x, rows);
+    if (lane == 31) scan[warp] = make_int3(x.x, x.y, rows);
     if (tid == 0) pick[0] = -1;
     if (tid < kThreads / 32 * kStages) barrier_init((unsigned)__cvta_generic_to_shared(&bars[0][0] + tid));
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    int before = x - mine;
+    int before = x.x - mine.x, before_short = x.y - mine.y;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-      const int2 got = scan[w];
+      const int3 got = scan[w];
+      before_short += got.x + (w < warp ? got.y : 0);                   // all the longer ones come first
       if (w < warp) before += got.x;
-      covered += got.y;
+      covered += got.z;
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int tiles = (count[i] + kItem - 1) / kItem, at = (item - before) * kItem;
-      if (item >= before && item < before + tiles) {
+      const int longer = (count[i] + kItem - 9) / kItem, shorter = (unsigned)(count[i] - 1) % kItem < 8 && count[i];
+      int at = -1;
+      if (item >= before && item < before + longer) at = (item - before) * kItem;
+      if (shorter && item == before_short) at = longer * kItem;
+      if (at >= 0) {
         pick[0] = tid * PER + i;
         pick[1] = first[i] + at;
         pick[2] = min(count[i] - at, kItem);
       }
-      before += tiles;
+      before += longer;
+      before_short += shorter;
     }
     __syncthreads();
   }
@@ -443,11 +455,12 @@ __global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_
     it.k_lo = (int)min(a.inner, rank * geo.slice);
     it.k_hi = (int)min(a.inner, it.k_lo + geo.slice);
     const unsigned bar = (unsigned)__cvta_generic_to_shared(&bars[0][0]);
-    switch ((it.rows + 7) / 8) {
-      case 1: item_sums<T, S, VEC, 1>(&map, a, geo, it, smem, bar); break;
-      case 2: item_sums<T, S, VEC, 2>(&map, a, geo, it, smem, bar); break;
-      case 3: item_sums<T, S, VEC, 3>(&map, a, geo, it, smem, bar); break;
-      default: item_sums<T, S, VEC, 4>(&map, a, geo, it, smem, bar); break;
+    const int columns = MOST == 1 ? 1 : (it.rows + 7) / 8;
+    if (columns == 1) item_sums<T, S, VEC, 1>(&map, a, geo, it, smem, bar);
+    else if constexpr (MOST > 1) {
+      if (columns == 2) item_sums<T, S, VEC, 2>(&map, a, geo, it, smem, bar);
+      else if (columns == 3) item_sums<T, S, VEC, 3>(&map, a, geo, it, smem, bar);
+      else item_sums<T, S, VEC, 4>(&map, a, geo, it, smem, bar);
     }
     // join the cluster's sums: CTA `rank` finishes every ranks-th part of the outputs
     float* sums = reinterpret_cast<float*>(smem + (kThreads / 32) * kStages * kTileBytes);
@@ -476,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_
     }
 }
 
-template <typename T, typename S, int VEC>
+template <typename T, typename S, int VEC, int MOST>
 cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
   // items: every segment's last may be partial
   const long long items = (a.rows + kItem - 1) / kItem + (a.segments < a.rows ? a.segments : a.rows) - 1;
@@ -499,7 +512,7 @@ cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
                              step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
-  auto kernel = int4_product_kernel<T, S, VEC>;
+  auto kernel = int4_product_kernel<T, S, VEC, MOST>;
   // the shared-memory limit is raised once per device and instance
   static std::atomic<unsigned long long> allowed{0};
   int device = 0;
@@ -525,16 +538,27 @@ cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
   return cudaLaunchKernelEx(&config, kernel, map, a, geo);
 }
 
+// up to 8 rows have one column: an instance without the others' registers (one token of 8 experts 19.3 us, not 20.4)
+template <typename T, typename S, int VEC>
+cudaError_t launch_columns(const Int4Args& a, cudaStream_t stream) {
+  return a.rows <= 8 ? launch<T, S, VEC, 1>(a, stream) : launch<T, S, VEC, 4>(a, stream);
+}
+
 template <typename T, typename S>
 cudaError_t launch_group(const Int4Args& a, cudaStream_t stream) {
-  if (a.group == 128) return launch<T, S, 4>(a, stream);
-  if (a.group == 64) return launch<T, S, 2>(a, stream);
-  return launch<T, S, 1>(a, stream);
+  if (a.group == 128) return launch_columns<T, S, 4>(a, stream);
+  if (a.group == 64) return launch_columns<T, S, 2>(a, stream);
+  return launch_columns<T, S, 1>(a, stream);
 }
 
 }  // namespace
 
-cudaError_t int4_late_copies(int* count) { return cudaMemcpyFromSymbol(count, late_copies, sizeof(int)); }
+cudaError_t int4_late_copies(int* flag) {
+  cudaError_t e = cudaMemcpyFromSymbol(flag, late_copies, sizeof(int));
+  const int none = 0;
+  if (e == cudaSuccess && *flag) e = cudaMemcpyToSymbol(late_copies, &none, sizeof(int));
+  return e;
+}
 
 cudaError_t launch_int4_product(const Int4Args& a, cudaStream_t stream) {
   if (a.rows == 0 || a.n == 0) return cudaSuccess;

@@ -224,6 +224,6 @@ struct Int4Args {
   long long out_stride;
 };
 cudaError_t launch_int4_product(const Int4Args& args, cudaStream_t stream);
-cudaError_t int4_late_copies(int* flag);   // 1 after a copy of any product that did not arrive in time
+cudaError_t int4_late_copies(int* flag);   // 1 if a copy of a product did not arrive in time since the last call
 
 }  // namespace vb

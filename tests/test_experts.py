@@ -488,6 +488,7 @@ def test_int4_product_matches_reference(dtype, wide_scales, rows, experts, activ
     # products and partial sums: at most inner additions, each of them and each group's scaling off by 2^-23 (the
     # matrix unit may cut instead of rounding)
     close(got, want, size, dtype, 2 * (inner + 3 * inner // group))
+    ex.check_status()
     # that bound is the worst case; the fp32 errors have random signs, so over all outputs they stay near the error
     # of one rounding of values as large as the partial sums (32 of which is 2^-19), far under the result's rounding
     assert (got.double() - want).norm() <= (half_step(dtype) + 2.0 ** -16) * want.norm()
@@ -644,3 +645,73 @@ def test_kernel_bench_runs_the_expert_kernels(kernel, capsys):
                               "--outputs", "48", "--group", "64", "--iters", "2"]) == 0
     line = json.loads(capsys.readouterr().out.strip().splitlines()[-1])
     assert line["us"] > 0 and kernel in line["kernel"]
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements of rows (and 2^32 bytes of weights): the last rows are where a 32-bit offset would wrap."""
+    g = cuda(41)
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    tokens, k, hidden = 270_000, 2, 4096
+    ids = torch.randint(0, 16, (tokens, k), device="cuda", generator=g, dtype=torch.int32)
+    order = ex.sort_by_expert(ids, 16)
+    x = torch.zeros(tokens, hidden, device="cuda", dtype=torch.bfloat16)
+    x[:, :8] = torch.randn(tokens, 8, device="cuda", generator=g).bfloat16()
+    rows = ex.dispatch(x, order)
+    source = order.source.long()
+    assert torch.equal(rows[:, :8], x[source // k, :8])
+    w = torch.full((tokens, k), 0.5, device="cuda")
+    assert torch.equal(ex.combine(rows, w, order), x)                 # two halves of the same value: exact
+    grad_rows, grad_w = ex.combine_backward(x, rows, w, order)
+    assert torch.equal(grad_rows[:, :8], (x * 0.5)[source // k, :8])
+    parts = x[:, :8].double().square()
+    close(grad_w, parts.sum(1, keepdim=True).expand(tokens, k), parts.sum(1, keepdim=True).expand(tokens, k),
+          torch.float32, 8)
+    assert torch.equal(ex.dispatch_backward(rows, order), (x.float() * 2).bfloat16())
+    del rows, grad_rows
+    experts, n, inner = 40, 16384, 16384                              # 5.4 GB of weights
+    packed = torch.full((experts, n, inner // 2), 0x88, dtype=torch.uint8, device="cuda")
+    packed[-1] = torch.randint(0, 256, (n, inner // 2), dtype=torch.uint8, device="cuda", generator=g)
+    scales = torch.ones(experts, n, inner // 128, device="cuda", dtype=torch.bfloat16)
+    counts = torch.zeros(experts, dtype=torch.int32, device="cuda")
+    counts[0], counts[-1] = 1, 2
+    starts = (counts.cumsum(0) - counts).int()
+    y = normal(g, 3, inner, dtype=torch.bfloat16)
+    got = ex.expert_matmul_int4(y, starts, counts, packed, scales)
+    assert bool((got[0] == 0).all())
+    q = torch.stack([packed[-1] & 15, packed[-1] >> 4], -1).flatten(-2).double() - 8
+    want, size = y[1:].double() @ q.T, y[1:].double().abs() @ q.abs().T
+    close(got[1:], want, size, torch.bfloat16, 2 * (inner + 3 * inner // 128))
+    assert (got[1:].double() - want).norm() <= (half_step(torch.bfloat16) + 2.0 ** -16) * want.norm()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls keep nothing between them: the same operators on two streams, many times, give the eager results."""
+    g = cuda(51)
+    work = []
+    for tokens, experts in ((700, 30), (41, 5)):
+        x, w = normal(g, tokens, 512, dtype=torch.bfloat16), torch.rand(tokens, 4, device="cuda", generator=g)
+        ids = torch.randint(0, experts, (tokens, 4), device="cuda", generator=g, dtype=torch.int32)
+        packed = torch.randint(0, 256, (experts, 256, 256), dtype=torch.uint8, device="cuda", generator=g)
+        scales = torch.rand(experts, 256, 8, device="cuda", generator=g).bfloat16()
+        work.append((x, w, ids, packed, scales, experts))
+
+    def step(x, w, ids, packed, scales, experts):
+        order = ex.sort_by_expert(ids, experts)
+        rows = ex.dispatch(x, order)
+        return ex.expert_matmul_int4(rows, order.starts, order.counts, packed, scales), ex.combine(rows, w, order)
+
+    want = [step(*w) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step(*work[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a in got[i]:
+            assert torch.equal(a[0], want[i][0]) and torch.equal(a[1], want[i][1])

@@ -380,7 +380,15 @@ def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.T
     segment per source rank and expert after an AllToAll), a multiple of the experts, at most 1024, that ascend
     and do not overlap; ``packed`` uint8 [experts, n, inner / 2] and ``scales`` [experts, n, inner / group] of the
     rows' dtype or float32, as :func:`quantize_int4` gives them, in groups of 32, 64 or 128.  Products and sums are
-    fp32, rounded once.  No gradients: 4-bit weights are for serving.
+    fp32, rounded once.  No gradients: 4-bit weights are for serving.  The kernel's waits are bounded: outputs whose
+    weights did not arrive in a second are NaN, and :func:`check_status` says so.
     """
     return _call("int4_product", lambda: _check_product(rows, starts, counts, packed, scales, out), rows, starts, counts,
                  packed, scales, out)
+
+
+def check_status() -> None:
+    """Raise when a 4-bit product on the current GPU gave up waiting for its weights since the last check (it waits
+    for the GPU; not for a stream that is being captured)."""
+    if _mod().int4_late_copies():
+        raise RuntimeFailure("a 4-bit product's copy of weights did not arrive in time; its outputs are NaN")

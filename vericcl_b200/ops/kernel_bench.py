@@ -149,6 +149,9 @@ def main(argv=None) -> int:
     t1.record(stream)
     torch.cuda.synchronize()
     comm.check_status()
+    if args.kernel == "expert_matmul_int4":
+        from vericcl_b200.ops import experts as ops
+        ops.check_status()
     us = t0.elapsed_time(t1) / args.iters * 1e3
     peak, source = hbm_peak_gbs()
     gbs = nbytes / (us * 1e-6) / 1e9
