@@ -79,7 +79,8 @@ Tensor cut(const Tensor& pool, int64_t offset, at::IntArrayRef sizes, at::Scalar
 void check_order(const Tensor& slot, const Tensor& source, const Tensor& like) {
   check_table(slot, like, at::kInt, "slot");
   check_table(source, like, at::kInt, "source");
-  TORCH_CHECK(slot.dim() == 2 && source.dim() == 1, "slot is [tokens, k], source [rows]");
+  TORCH_CHECK(slot.dim() == 2 && source.dim() == 1 && slot.size(1) >= 1 && slot.size(1) <= kMaxChoices,
+              "slot is [tokens, k], source [rows]");
   TORCH_CHECK(slot.numel() <= INT_MAX && source.numel() <= INT_MAX, "more than 2^31 - 1 assignments or rows");
 }
 

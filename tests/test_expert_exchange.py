@@ -105,7 +105,7 @@ class Threads:
         self.world, self.gate, self.parts = world, threading.Barrier(world, timeout=60), {}
 
     def engine(self, rank):
-        comm = SimpleNamespace(world=self.world, rank=rank, free=lambda t: None,
+        comm = SimpleNamespace(world=self.world, rank=rank, device=0, free=lambda t: None,
                                empty=lambda n, dtype=torch.float32: torch.empty(n, dtype=dtype, device="cuda"))
 
         def all_to_all(inp, out):

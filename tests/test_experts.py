@@ -60,6 +60,8 @@ REFUSED = [
     lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order(), out=torch.zeros(5, 8)),
     lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order(), out=torch.zeros(6, 8, dtype=torch.float16)),
     lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order(), out=torch.zeros(1, 8).expand(6, 8)),
+    lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order(k=33, rows=99)),
+    lambda: ex.dispatch(torch.zeros(3, 8), _cpu_order(k=0)),
     lambda: ex.dispatch_backward(torch.zeros(5, 8), _cpu_order()),
     lambda: ex.combine(torch.zeros(5, 8), torch.zeros(3, 2), _cpu_order()),
     lambda: ex.combine(torch.zeros(6, 8), torch.zeros(3, 2, dtype=torch.bfloat16), _cpu_order()),
@@ -70,6 +72,7 @@ REFUSED = [
     lambda: ex.quantize_int4(torch.zeros(8)),
     lambda: ex.quantize_int4(torch.zeros(8, 100), 32),
     lambda: ex.quantize_int4(torch.zeros(8, 96), 48),
+    lambda: ex.quantize_int4(torch.full((8, 32), float("nan")), 32),
     lambda: ex.quantize_int4(torch.zeros(8, 128), 128, scale_dtype=torch.float64),
 ]
 
@@ -715,3 +718,23 @@ def test_two_streams_at_once():
     for i in range(2):
         for a in got[i]:
             assert torch.equal(a[0], want[i][0]) and torch.equal(a[1], want[i][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_route_infinity_is_chosen_and_spoils_the_weights(renormalize):
+    cuda()
+    ids, w = ex.route(torch.tensor([[1.0, math.inf, 2]], device="cuda"), 2, renormalize=renormalize)
+    assert ids.tolist() == [[1, 2]] and bool(w.isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts,k", [(128, 8), (300, 16), (1000, 32)])
+def test_route_many_equal_logits(experts, k):
+    """Few distinct values: more candidates than a warp has lanes, ties everywhere."""
+    g = cuda(experts)
+    logits = torch.randint(0, 3, (50, experts), device="cuda", generator=g).to(torch.bfloat16)
+    logits[:10] = 1.0
+    logits[10:20, k // 2:] = -math.inf
+    ids, _ = ex.route(logits, k)
+    assert torch.equal(ids, reference_route(logits, k, True)[0])

@@ -45,7 +45,7 @@ class ExpertExchange:
         self.rows = experts * capacity
         self.order = None
         self._heap: dict = {}
-        segments = torch.arange(experts, dtype=torch.int32, device="cuda")
+        segments = torch.arange(experts, dtype=torch.int32, device=torch.device("cuda", comm.device))
         self.starts = segments * capacity
         self.counts = torch.zeros_like(segments)
 

@@ -96,6 +96,8 @@ def _order(order):
     if slot.dtype != torch.int32 or slot.dim() != 2 or not slot.is_contiguous() or \
             source.dtype != torch.int32 or source.dim() != 1 or not source.is_contiguous():
         raise RuntimeFailure("an order holds contiguous int32 slot [tokens, k] and source [rows]")
+    if not 1 <= slot.size(1) <= MAX_CHOICES or max(slot.numel(), source.numel()) > _INT_MAX:
+        raise RuntimeFailure("an order has 1 to %d choices, and fewer than 2^31 assignments and rows" % MAX_CHOICES)
     return slot, source
 
 
@@ -172,7 +174,7 @@ def route(logits: torch.Tensor, k: int, *, renormalize: bool = True):
     ``renormalize=False`` their share of the softmax over all.
 
     A logit of -inf takes its expert out: a token with fewer than ``k`` experts left gets id -1 and weight 0 for
-    the rest.  A NaN logit is never chosen and makes the weights of its token NaN.
+    the rest.  A NaN logit is never chosen and makes the weights of its token NaN, and so does +inf, which is.
     """
     if logits.requires_grad and _learns():
         return _Route.apply(logits, k, renormalize)
@@ -327,7 +329,8 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, scale_dtype: torch.
 
     Value ``k`` of a row is ``(q - 8) * scale``: two 4-bit ``q`` a byte, the even ``k`` in the low half.  The scale of
     a group, its largest magnitude / 7, is rounded to ``scale_dtype`` (the weight's by default) before the values
-    are, so its rounding moves the grid and adds no error of its own.  Done once when weights are loaded.
+    are, so its rounding moves the grid and adds no error of its own but to a largest magnitude that it leaves
+    beyond 7 steps, which is clamped.  Weights must be finite.  Done once when they are loaded.
     """
     if weight.dim() < 2 or weight.dtype not in _DTYPES:
         raise RuntimeFailure("a weight is [..., n, inner] of float32, bfloat16 or float16")
@@ -337,6 +340,8 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, scale_dtype: torch.
     if dtype not in _DTYPES:
         raise RuntimeFailure("scales are float32, bfloat16 or float16")
     w = weight.detach().float().unflatten(-1, (-1, group))
+    if not bool(torch.isfinite(w).all()):
+        raise RuntimeFailure("a weight to quantize holds infinities or NaN")
     scales = (w.abs().amax(-1) / 7.0).to(dtype)
     scales = torch.where(scales == 0, torch.ones_like(scales), scales)      # a group of zeros
     q = (torch.round(w / scales.float()[..., None]).clamp_(-8, 7) + 8).to(torch.uint8).flatten(-2)
