@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
 // vectors take 4 a lane (fp32 rows of 1030: dispatch 22.0 us, with 2 23.2).
 //
 // Rows that together exceed half of the L2 are read and written as streams (evicted first), as they will not be
-// found there again: 8192 x 8 x 2048 bf16 dispatch 50.9 -> 46.9 us, combine 53.7 -> 46.8, its gradient 109 -> 105.
+// found there again: 8192 x 8 x 2048 bf16 dispatch 50.9 -> 46.9 us, combine 53.7 -> 46.8, its gradient 109 -> 105 us.
 // Smaller ones stay for the kernel that follows.
 template <int BYTES> constexpr int kPieces = BYTES == 16 ? 2 : 4;
 constexpr int kRowWarps = 8;
@@ -549,9 +549,11 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(ExchangeRowsArg
 }
 
 // One CTA per token, its warps share the pieces: a piece of the gradient is read once and multiplied with and into
-// each of the token's rows.  The products of the pieces are added in a fixed order.
+// each of the token's rows.  The products of the pieces are added in a fixed order.  Many rows are held to 64
+// registers a thread for their warps' sake (8192 x 8 x 2048 bf16: 106 -> 98.5 us), few are faster without (256 x 8 x
+// 4096: 6.0 us, held 6.8).
 template <typename T, int N, bool STREAM>
-__global__ void __launch_bounds__(kRowWarps * 32) combine_backward_kernel(ExchangeRowsArgs a, long long units, unsigned token_blocks) {
+__global__ void __launch_bounds__(kRowWarps * 32, STREAM ? 4 : 1) combine_backward_kernel(ExchangeRowsArgs a, long long units, unsigned token_blocks) {
   using V = Vec<T, N>;
   constexpr int P = kPieces<sizeof(V)>;
   __shared__ float part[kRowWarps][kMaxChoices];
