@@ -3,17 +3,23 @@
 // for the rows r of expert e's segments.
 //
 // The weights are read once and are what bounds a few rows, so a weight may cost little more than one
-// instruction.  Eight 4-bit values of a word become four registers of two 16-bit numbers each (mask, or in an
-// exponent, subtract: exact in bf16 and fp16), which are fragments of a 16 x 16 matrix-unit product with up to
-// 8 rows of x as the other side; its sums are fp32.  One group's sum is scaled in fp32 and added to the total,
-// so a scale is never rounded into a weight.
+// instruction.  Eight 4-bit values of a word become four registers of two 16-bit numbers each, in nine instructions,
+// which are fragments of a 16 x 16 matrix-unit product with up to 8 rows of x as the other side; its sums are fp32.
+// One group's sum is scaled in fp32 and added to the total, so a scale is never rounded into a weight.
 //
-// A CTA of 8 warps covers 128 weight rows, 16 a warp.  Every warp streams its rows through its own ring of 2 KB
-// tiles (16 rows of 128 bytes, 256 inner values) that TMA fills, so no warp waits for another and the bytes in
-// flight cost no registers.  A lane holds, of two weight rows and of every group, the group / 4 values from
-// (lane % 4) * group / 4 on; x is staged in shared memory in that order, so its fragment is one conflict-free
-// 16-byte load.  A cluster of 1 to 8 CTAs splits the inner size and joins its fp32 sums through distributed
-// shared memory in the order of the CTAs.
+// A CTA of 8 warps covers 128 weight rows, 16 a warp, and two CTAs share an SM.  Every warp streams its rows through
+// its own ring of two 4 KB tiles (16 rows of 256 bytes, 512 inner values) that TMA fills, so no warp waits for
+// another and the bytes in flight (128 KB of an SM) cost no registers.  A lane holds, of two weight rows and of every
+// group, the group / 4 values from (lane % 4) * group / 4 on; x is staged in shared memory in that order, so its
+// fragment is one conflict-free 16-byte load.  A cluster of 1 to 8 CTAs splits the inner size where the CTAs would
+// not fill the GPU and joins its fp32 sums through distributed shared memory in the order of the CTAs.
+//
+// One row for each of 8 experts 4096 x 4096 (69 MB): 20.6 us, 3.3 TB/s.  The same kernel takes 15 us without its
+// arithmetic and 14 without its loads, so what is left is that the two overlap only in part: the arithmetic keeps
+// its integer pipe 60 % busy, and 16 warps of an SM are what its registers and ring allow.  Measured and not kept:
+// three CTAs of fewer registers (24.5 us), a barrier per 2 KB box (22.8), and one CTA per SM walking equal runs of
+// strips (26.8).  From about 16 rows an expert on the matrix unit bounds it: 1024 rows of 8 experts 1024 x 2048 take
+// 30.9 us, 139 TFLOP/s.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -163,18 +169,16 @@ __device__ __forceinline__ void load_scales(float (&f)[PAIR], const S* s) {
   }
 }
 
-// PAIR groups of 16 weight rows times COLS x 8 rows of x, scaled and added to acc.  `x` is the lane's first unit, the
-// next word's is `step` units further (32 * COLS, or with one column 4 times its rows rounded to a power of two);
-// `scale` points to the lane's first weight row, the second is `second` further.
-// The groups' products alternate, and with one column and longer groups each group's sum is kept in two halves, so that a product
-// seldom waits for the one before it.  A lane whose row of x does not exist computes with what lies there: columns
-// of a product do not mix, and that column is not written.
+// PAIR groups of 16 weight rows times COLS x 8 rows of x, scaled and added to acc; the groups' products alternate, so
+// that a product seldom waits for the one before it.  `x` is the lane's first unit, the next word's is `step` units
+// further (32 * COLS, or with one column 4 times its rows rounded to a power of two); `scale` points to the lane's
+// first weight row, the second is `second` further.  A lane whose row of x does not exist computes with what lies
+// there: columns of a product do not mix, and that column is not written.
 template <typename T, typename S, int VEC, int COLS, int PAIR>
 __device__ __forceinline__ void group_product(float (&acc)[COLS][4], const unsigned char* tile, unsigned at, int u0,
                                               const uint4* x, int step, const S* scale, int second) {
-  constexpr int HALVES = COLS == 1 && VEC > 1 ? 2 : 1;
   unsigned ra[PAIR][VEC], rb[PAIR][VEC];
-  float part[PAIR][HALVES][COLS][4];
+  float part[PAIR][COLS][4];
 #pragma unroll
   for (int p = 0; p < PAIR; ++p) {
     // within a box the groups differ in the chunk bits, which the swizzle leaves to an exclusive or
@@ -193,8 +197,8 @@ __device__ __forceinline__ void group_product(float (&acc)[COLS][4], const unsig
 #pragma unroll
       for (int t = 0; t < COLS; ++t) {
         const uint4 b = x[(p * VEC + v) * (COLS == 1 ? step : 32 * COLS) + t * 32];
-        mma<T>(part[p][0][t], va, vb, 0, b.x, b.y, v == 0);
-        mma<T>(part[p][HALVES - 1][t], va, vb, 2, b.z, b.w, HALVES == 2 && v == 0);
+        mma<T>(part[p][t], va, vb, 0, b.x, b.y, v == 0);
+        mma<T>(part[p][t], va, vb, 2, b.z, b.w, false);
       }
     }
   float first[PAIR], other[PAIR];
@@ -206,11 +210,7 @@ __device__ __forceinline__ void group_product(float (&acc)[COLS][4], const unsig
 #pragma unroll
     for (int t = 0; t < COLS; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float sum = part[p][0][t][i];
-        if constexpr (HALVES == 2) sum += part[p][1][t][i];
-        acc[t][i] = fmaf(i < 2 ? sa : sb, sum, acc[t][i]);
-      }
+      for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(i < 2 ? sa : sb, part[p][t][i], acc[t][i]);
   }
 }
 
@@ -337,7 +337,8 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
         if (late < 0 && !__all_sync(kFull, wait_tile(bar + 8 * slot, phase))) late = (c0 + u0) / UNITS;
         const unsigned char* tile = ring + slot * kTileBytes;
         if (u0 + UNITS <= here) {
-#pragma unroll
+          // unrolled with one column only: with more the registers spill (1024 rows of 8 experts 32.7 us, so 28.8)
+#pragma unroll (COLS == 1 ? UNITS : 1)
           for (int u = 0; u < UNITS; u += PAIR)
             group_product<T, S, VEC, COLS, PAIR>(acc, tile, lane_at, u, xw + u * VEC * step, step, sw + u, 8 * pitch);
         } else {
