@@ -738,3 +738,26 @@ def test_route_many_equal_logits(experts, k):
     logits[10:20, k // 2:] = -math.inf
     ids, _ = ex.route(logits, k)
     assert torch.equal(ids, reference_route(logits, k, True)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,scale_dtype", [(32, torch.float32), (64, torch.float16), (128, torch.float16)])
+def test_int4_product_segments_in_any_order_and_of_all_lengths(group, scale_dtype):
+    """Segments of 0, 1, 8, 9, 32, 33, 41 and 65 rows, later ones first: every number of columns, items that are
+    sorted by their length, and more than one stage of x and scales."""
+    g = cuda(group)
+    lengths = [65, 0, 9, 33, 1, 41, 32, 8]
+    starts, at = [0] * 8, 0
+    for s in reversed(range(8)):
+        starts[s] = at
+        at += lengths[s]
+    inner = 5 * 512 + group                                           # the last tile holds one group
+    i32 = dict(dtype=torch.int32, device="cuda")
+    starts, counts = torch.tensor(starts, **i32), torch.tensor(lengths, **i32)
+    x = normal(g, at, inner, dtype=torch.float16)
+    packed = torch.randint(0, 256, (4, 145, inner // 2), dtype=torch.uint8, device="cuda", generator=g)
+    scales = (0.01 + 0.02 * torch.rand(4, 145, inner // group, device="cuda", generator=g)).to(scale_dtype)
+    got = ex.expert_matmul_int4(x, starts, counts, packed, scales)
+    want, size = product_reference(x, starts, counts, packed, scales, group)
+    close(got, want, size, torch.float16, 2 * (inner + 3 * inner // group))
+    assert (got.double() - want).norm() <= (half_step(torch.float16) + 2.0 ** -16) * want.norm()
