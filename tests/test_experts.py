@@ -761,3 +761,21 @@ def test_int4_product_segments_in_any_order_and_of_all_lengths(group, scale_dtyp
     want, size = product_reference(x, starts, counts, packed, scales, group)
     close(got, want, size, torch.float16, 2 * (inner + 3 * inner // group))
     assert (got.double() - want).norm() <= (half_step(torch.float16) + 2.0 ** -16) * want.norm()
+
+
+@pytest.mark.gpu
+def test_gradients_of_broadcast_tokens_and_of_expanded_gradients():
+    """One row of x for every token (its gradient is the sum over them), and a gradient that is one number expanded."""
+    g = cuda(61)
+    base, w = normal(g, 1, 40).requires_grad_(), torch.rand(7, 2, device="cuda", generator=g).requires_grad_()
+    order = ex.sort_by_expert(random_ids(g, 7, 2, 3), 3)
+    rows = ex.dispatch(base.expand(7, 40), order)
+    out = ex.combine(rows, w, order)
+    out.sum().backward()
+    kept = (order.slot >= 0).double()
+    share = (w.detach().double() * kept).sum()
+    # every row adds its weight once: sums of 14 positive terms, each addition off by 2^-24 of at most the sum
+    assert bool(((base.grad.double() - share).abs() <= 32 * 2.0 ** -24 * share).all())
+    total = base.detach().double().sum()
+    size = base.detach().double().abs().sum()
+    assert bool(((w.grad.double() - kept * total).abs() <= 41 * 2.0 ** -24 * size).all())
