@@ -416,8 +416,8 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_kernel(SortArgs a) {
 // All three kernels are bound by the bytes they move.  A warp moves a piece of 2 or 4 vectors a lane of one token
 // to or from the token's rows: the token's side is read or written once however many rows it has, and the piece's
 // vectors are all in flight together.  Vectors are the widest (16, 8 bytes or one element) that every address,
-// stride and row length allows; blockIdx.y is the piece, so no index is divided.  Blocks past the tokens' clear the
-// rows that have no token.
+// stride and row length allows; blockIdx.y is the piece, so no index is divided.  The grid's first
+// blocks clear the rows that have no token.
 //
 // A piece is 1 KB of 16-byte vectors.  Longer pieces, or rows requested ahead, cost registers and with them the
 // warps that hide the latency: combining 8192 tokens x 8 rows x 2048 bf16 takes 53.7 us with 2 vectors a lane, 62.2
@@ -457,31 +457,38 @@ __device__ __forceinline__ uint2 zero_vec(uint2) { return make_uint2(0, 0); }
 __device__ __forceinline__ unsigned zero_vec(unsigned) { return 0; }
 __device__ __forceinline__ unsigned short zero_vec(unsigned short) { return 0; }
 
-// rows of `source` without an assignment, 32 a warp; `block` counts from the first block past the tokens'
+// Rows of `source` without an assignment, 32 a warp: the warps of the first `blocks` blocks take every row in turn, as
+// the empty rows of an expert lie together and 32 of them at one warp would outlast the copies (30720 rows of 1030
+// fp32, 9000 of them empty: 31 us, so 27).
+__device__ __forceinline__ unsigned empty_rows(const ExchangeRowsArgs& a, unsigned blocks, long long& first, long long& step) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  first = (long long)blockIdx.x * warps + (threadIdx.x >> 5);
+  step = (long long)blocks * warps;
+  const long long r = first + lane * step;
+  return __ballot_sync(kFull, r < a.rows && a.source[r] < 0);
+}
+
 template <typename V>
-__device__ __forceinline__ void clear_rows(const ExchangeRowsArgs& a, V* out, long long stride, long long block, long long units) {
-  const int lane = threadIdx.x & 31;
-  const long long r0 = (block * (blockDim.x >> 5) + (threadIdx.x >> 5)) * 32;
+__device__ __forceinline__ void clear_rows(const ExchangeRowsArgs& a, V* out, long long stride, unsigned blocks, long long units) {
   constexpr int P = kPieces<sizeof(V)>;
-  const long long c0 = (long long)blockIdx.y * (32 * P) + lane;
-  unsigned empty = __ballot_sync(kFull, r0 + lane < a.rows && a.source[r0 + lane] < 0);
-  while (empty) {
-    const long long r = r0 + __ffs(empty) - 1;
-    empty &= empty - 1;
+  const long long c0 = (long long)blockIdx.y * (32 * P) + (threadIdx.x & 31);
+  long long first, step;
+  for (unsigned empty = empty_rows(a, blocks, first, step); empty; empty &= empty - 1) {
+    V* to = out + (first + (__ffs(empty) - 1) * step) * stride + c0;
 #pragma unroll
     for (int i = 0; i < P; ++i)
-      if (c0 + 32 * i < units) out[r * stride + c0 + 32 * i] = zero_vec(V{});
+      if (c0 + 32 * i < units) to[32 * i] = zero_vec(V{});
   }
 }
 
 // V-sized vectors; strides and lengths are in vectors
 template <typename V, bool STREAM>
-__global__ void __launch_bounds__(kRowWarps * 32) dispatch_kernel(ExchangeRowsArgs a, long long units, unsigned token_blocks) {
+__global__ void __launch_bounds__(kRowWarps * 32) dispatch_kernel(ExchangeRowsArgs a, long long units, unsigned clear_blocks) {
   const V* in = static_cast<const V*>(a.in);
   V* out = static_cast<V*>(a.out);
-  if (blockIdx.x >= token_blocks) { clear_rows(a, out, a.out_stride, blockIdx.x - token_blocks, units); return; }
+  if (blockIdx.x < clear_blocks) { clear_rows(a, out, a.out_stride, clear_blocks, units); return; }
   const int lane = threadIdx.x & 31;
-  const long long t = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  const long long t = (long long)(blockIdx.x - clear_blocks) * kRowWarps + (threadIdx.x >> 5);
   if (t >= a.tokens) return;
   const int mine = lane < a.k ? a.slot[t * a.k + lane] : -1;
   constexpr int P = kPieces<sizeof(V)>;
@@ -553,23 +560,24 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(ExchangeRowsArg
 // registers a thread for their warps' sake (8192 x 8 x 2048 bf16: 106 -> 98.5 us), few are faster without (256 x 8 x
 // 4096: 6.0 us, held 6.8).
 template <typename T, int N, bool STREAM>
-__global__ void __launch_bounds__(kRowWarps * 32, STREAM ? 4 : 1) combine_backward_kernel(ExchangeRowsArgs a, long long units, unsigned token_blocks) {
+__global__ void __launch_bounds__(kRowWarps * 32, STREAM ? 4 : 1) combine_backward_kernel(ExchangeRowsArgs a, long long units, unsigned clear_blocks) {
   using V = Vec<T, N>;
   constexpr int P = kPieces<sizeof(V)>;
   __shared__ float part[kRowWarps][kMaxChoices];
   V* out = static_cast<V*>(a.out);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  if (blockIdx.x >= token_blocks) {     // 32 rows a warp, every piece of them
-    const long long r0 = ((long long)(blockIdx.x - token_blocks) * warps + warp) * 32;
-    unsigned empty = __ballot_sync(kFull, r0 + lane < a.rows && a.source[r0 + lane] < 0);
+  if (blockIdx.x < clear_blocks) {      // every piece of the rows
     V zero;
 #pragma unroll
     for (int n = 0; n < N; ++n) zero.v[n] = from_f<T>(0.f);
-    for (; empty; empty &= empty - 1)
-      for (long long c = lane; c < units; c += 32) out[(r0 + __ffs(empty) - 1) * a.out_stride + c] = zero;
+    long long first, step;
+    for (unsigned empty = empty_rows(a, clear_blocks, first, step); empty; empty &= empty - 1) {
+      V* to = out + (first + (__ffs(empty) - 1) * step) * a.out_stride;
+      for (long long c = lane; c < units; c += 32) to[c] = zero;
+    }
     return;
   }
-  const long long t = blockIdx.x;
+  const long long t = blockIdx.x - clear_blocks;
   int mine = -1;
   float weight = 0.f, dots = 0.f;       // lane j: choice j
   if (lane < a.k) {
@@ -694,7 +702,7 @@ cudaError_t dispatch_as(ExchangeRowsArgs a, cudaStream_t stream) {
   const unsigned clear_blocks = (unsigned)((a.rows + 32 * kRowWarps - 1) / (32 * kRowWarps));
   if (pieces > 65535) return cudaErrorInvalidConfiguration;
   auto kernel = streamed ? dispatch_kernel<V, true> : dispatch_kernel<V, false>;
-  kernel<<<dim3(token_blocks + clear_blocks, (unsigned)pieces), kRowWarps * 32, 0, stream>>>(a, a.hidden, token_blocks);
+  kernel<<<dim3(token_blocks + clear_blocks, (unsigned)pieces), kRowWarps * 32, 0, stream>>>(a, a.hidden, clear_blocks);
   return cudaGetLastError();
 }
 
@@ -717,7 +725,7 @@ cudaError_t combine_backward_as(ExchangeRowsArgs a, cudaStream_t stream) {
   const unsigned clear_blocks = (unsigned)((a.rows + 32 * warps - 1) / (32 * warps));
   if (a.tokens + clear_blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   auto kernel = streamed ? combine_backward_kernel<T, N, true> : combine_backward_kernel<T, N, false>;
-  kernel<<<(unsigned)a.tokens + clear_blocks, warps * 32, 0, stream>>>(a, a.hidden, (unsigned)a.tokens);
+  kernel<<<(unsigned)a.tokens + clear_blocks, warps * 32, 0, stream>>>(a, a.hidden, clear_blocks);
   return cudaGetLastError();
 }
 
