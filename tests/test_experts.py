@@ -779,3 +779,35 @@ def test_gradients_of_broadcast_tokens_and_of_expanded_gradients():
     total = base.detach().double().sum()
     size = base.detach().double().abs().sum()
     assert bool(((w.grad.double() - kept * total).abs() <= 41 * 2.0 ** -24 * size).all())
+
+
+@pytest.mark.parametrize("weight_dtype,scale_dtype,magnitude", [
+    (torch.float32, torch.float16, 1e6), (torch.bfloat16, torch.float16, 1e6), (torch.float32, torch.float16, 7 * 65520.0)])
+def test_quantize_int4_refuses_scales_beyond_their_type(weight_dtype, scale_dtype, magnitude):
+    """65520 is the lowest magnitude that rounds to fp16's infinity."""
+    w = torch.ones(2, 128, dtype=weight_dtype)
+    w[1, 70] = magnitude
+    with pytest.raises(RuntimeFailure, match="range"):
+        ex.quantize_int4(w, 64, scale_dtype=scale_dtype)
+    packed, scales = ex.quantize_int4(w, 64, scale_dtype=torch.float32)          # a wider type holds it
+    assert bool(scales.isfinite().all())
+    w[1, 70] = 7 * 65000.0                                                       # near the largest fp16 value, 65504
+    assert 64000 < ex.quantize_int4(w, 64, scale_dtype=scale_dtype)[1][1, 1] <= 65504
+
+
+@pytest.mark.parametrize("dtype,scale_dtype", [(torch.float16, torch.float16), (torch.float32, torch.float16),
+                                               (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32),
+                                               (torch.float32, torch.bfloat16)])
+def test_quantize_int4_keeps_groups_whose_scale_underflows(dtype, scale_dtype):
+    """Magnitudes of at most 3.5 smallest scales: their seventh rounds to 0, and the smallest positive scale holds
+    them to half a step.  A group of zeros stays zeros."""
+    least = torch.finfo(scale_dtype).smallest_normal * torch.finfo(scale_dtype).eps
+    w = torch.zeros(3, 64, dtype=torch.float64)
+    w[0, :32] = torch.linspace(-3.0, 3.0, 32, dtype=torch.float64) * least
+    w[1, 3] = least
+    w = w.to(dtype)
+    packed, scales = ex.quantize_int4(w, 32, scale_dtype=scale_dtype)
+    assert bool((scales > 0).all()) and scales[0, 0] == least and scales[1, 0] == least
+    back = dequantized(packed, scales, 32)
+    assert bool(((back - w.double()).abs() <= least * 0.5).all())
+    assert bool((back[2] == 0).all()) and back[1, 3] == least

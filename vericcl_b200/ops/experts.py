@@ -330,7 +330,9 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, scale_dtype: torch.
     Value ``k`` of a row is ``(q - 8) * scale``: two 4-bit ``q`` a byte, the even ``k`` in the low half.  The scale of
     a group, its largest magnitude / 7, is rounded to ``scale_dtype`` (the weight's by default) before the values
     are, so its rounding moves the grid and adds no error of its own but to a largest magnitude that it leaves
-    beyond 7 steps, which is clamped.  Weights must be finite.  Done once when they are loaded.
+    beyond 7 steps, which is clamped.  A scale that would round to 0 is the smallest positive value instead (1 in a
+    group of zeros); one beyond the range of ``scale_dtype`` is refused.  Weights must be finite.  Done once when they
+    are loaded.
     """
     if weight.dim() < 2 or weight.dtype not in _DTYPES:
         raise RuntimeFailure("a weight is [..., n, inner] of float32, bfloat16 or float16")
@@ -342,8 +344,12 @@ def quantize_int4(weight: torch.Tensor, group: int = 128, *, scale_dtype: torch.
     w = weight.detach().float().unflatten(-1, (-1, group))
     if not bool(torch.isfinite(w).all()):
         raise RuntimeFailure("a weight to quantize holds infinities or NaN")
-    scales = (w.abs().amax(-1) / 7.0).to(dtype)
-    scales = torch.where(scales == 0, torch.ones_like(scales), scales)      # a group of zeros
+    largest = w.abs().amax(-1)
+    scales = (largest / 7.0).to(dtype)
+    if not bool(torch.isfinite(scales).all()):
+        raise RuntimeFailure("a group's largest magnitude / 7 is beyond the range of %s scales" % dtype)
+    least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps     # the smallest subnormal
+    scales = torch.where(scales == 0, torch.full_like(scales, least).masked_fill_(largest == 0, 1.0), scales)
     q = (torch.round(w / scales.float()[..., None]).clamp_(-8, 7) + 8).to(torch.uint8).flatten(-2)
     return (q[..., 0::2] | (q[..., 1::2] << 4)).contiguous(), scales.contiguous()
 
