@@ -193,3 +193,48 @@ def test_int4_products_of_exchanged_rows():
             # one weight (1.0), one rounding of the product; fp32 sums of 64 terms
             size = dense[ids[t, 0]].abs() @ x[t].double().abs()
             assert bool(((out[t].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -15 * size).all())
+
+
+def alone(**kwargs):
+    """An exchange of one rank without a communicator's heap."""
+    comm = SimpleNamespace(world=1, rank=0, device=0, free=lambda t: None,
+                           empty=lambda n, dtype=torch.float32: torch.empty(n, dtype=dtype, device="cuda"))
+    return ExpertExchange(SimpleNamespace(comm=comm), **kwargs)
+
+
+@pytest.mark.gpu
+def test_gradients_of_another_dispatch_are_refused():
+    gpu()
+    exchange = alone(experts=4, hidden=16, capacity=8, dtype=torch.float32)
+    x, logits, grad = tokens_for(0, 6, 4, 2, 16, torch.float32)
+    ids, w = ex.route(logits, 2)
+    other = (ids + 1) % 4
+
+    def forward(choices):
+        rows = exchange.dispatch(x, choices)
+        return exchange.combine(rows * 2, w)
+
+    forward(ids)
+    want_rows, want_w = (t.clone() for t in exchange.combine_backward(grad, w))
+    want_x = exchange.dispatch_backward(want_rows * 2)
+    # a dispatch between combine and its gradient
+    exchange.dispatch(x, other)
+    with pytest.raises(RuntimeFailure, match="combine"):
+        exchange.combine_backward(grad, w)
+    # between the gradient of combine and that of dispatch
+    forward(ids)
+    grad_rows = exchange.combine_backward(grad, w)[0].clone()
+    exchange.dispatch(x, other)
+    with pytest.raises(RuntimeFailure, match="dispatch"):
+        exchange.dispatch_backward(grad_rows * 2)
+    # the next step has its own
+    forward(other)
+    exchange.combine_backward(grad, w)
+    forward(ids)
+    got_rows, got_w = exchange.combine_backward(grad, w)
+    assert torch.equal(got_rows, want_rows) and torch.equal(got_w, want_w)
+    assert torch.equal(exchange.dispatch_backward(got_rows * 2), want_x)
+    # without a combine, the gradient of dispatch is that of the last one
+    exchange.dispatch(x, other)
+    direct = exchange.dispatch_backward(torch.ones(32, 16, device="cuda"))
+    assert torch.equal(direct, (exchange.order.slot >= 0).sum(1, keepdim=True).float().expand(6, 16))

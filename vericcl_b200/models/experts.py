@@ -44,6 +44,8 @@ class ExpertExchange:
         self.experts, self.hidden, self.capacity, self.dtype = experts, hidden, capacity, dtype
         self.rows = experts * capacity
         self.order = None
+        self._returned = None        # rows of the last combine, until another dispatch
+        self._grad_of = None         # the order of a combine gradient whose dispatch gradient is to come
         self._heap: dict = {}
         segments = torch.arange(experts, dtype=torch.int32, device=torch.device("cuda", comm.device))
         self.starts = segments * capacity
@@ -94,11 +96,11 @@ class ExpertExchange:
         """Rows of this rank's experts from every rank's tokens ``x`` [tokens, hidden] and choices ``ids`` [tokens, k].
 
         Ranks may hold different numbers of tokens; a choice beyond an expert's ``capacity`` rows is dropped
-        (``order.slot`` is -1 there)."""
+        (``order.slot`` is -1 there).  The gradients of an earlier ``combine`` and dispatch end here."""
         self._check_tokens(x, "x")
         if self.comm.world > 1 and self.capacity > 1 << 24:
             raise RuntimeFailure("a capacity above 2^24 cannot be exchanged")
-        self.order = ops.sort_by_expert(ids, self.experts, capacity=self.capacity)
+        self.order, self._returned = ops.sort_by_expert(ids, self.experts, capacity=self.capacity), None
         rows = ops.dispatch(x.detach(), self.order, out=self._buffer("sent"))
         self.counts = self._exchange_counts(self.order.counts)
         return self._exchange(rows, "received")
@@ -123,17 +125,23 @@ class ExpertExchange:
         its tokens' weights.  On one rank the rows given to ``combine`` must still hold."""
         order = self._dispatched()
         self._check_tokens(grad_out, "grad_out")
-        if getattr(self, "_returned", None) is None:
-            raise RuntimeFailure("combine comes before its gradient")
+        if self._returned is None:
+            raise RuntimeFailure("combine comes before its gradient, without another dispatch between them")
         grad, grad_weights = ops.combine_backward(grad_out, self._returned, weights.detach(), order,
                                                   out=self._buffer("grad_sent"))
+        self._grad_of = order
         return self._exchange(grad, "grad_received"), grad_weights
 
     def dispatch_backward(self, grad_rows: torch.Tensor) -> torch.Tensor:
-        """Gradient of ``x`` [tokens, hidden] from the gradient of the dispatched rows."""
+        """Gradient of the last :meth:`dispatch`'s ``x`` [tokens, hidden] from the gradient of its rows; refused when
+        that dispatch came after the :meth:`combine_backward` whose rows' gradient is on its way."""
         order = self._dispatched()
         self._check_rows(grad_rows, "grad_rows")
-        return ops.dispatch_backward(self._exchange(grad_rows, "grad_returned"), order)
+        if self._grad_of is not None and self._grad_of is not order:
+            raise RuntimeFailure("another dispatch came between the gradients of combine and dispatch")
+        grad = ops.dispatch_backward(self._exchange(grad_rows, "grad_returned"), order)
+        self._grad_of = None
+        return grad
 
     def close(self) -> None:
         """Give the heap buffers back (no exchange may be in flight)."""
@@ -141,4 +149,4 @@ class ExpertExchange:
             for t in buf if isinstance(buf, tuple) else (buf,):
                 self.comm.free(t)
         self._heap.clear()
-        self.order = self._returned = None
+        self.order = self._returned = self._grad_of = None
