@@ -238,3 +238,22 @@ def test_gradients_of_another_dispatch_are_refused():
     exchange.dispatch(x, other)
     direct = exchange.dispatch_backward(torch.ones(32, 16, device="cuda"))
     assert torch.equal(direct, (exchange.order.slot >= 0).sum(1, keepdim=True).float().expand(6, 16))
+
+
+@pytest.mark.gpu
+def test_a_refused_call_leaves_the_exchange_as_it_was():
+    gpu()
+    exchange = alone(experts=4, hidden=16, capacity=8, dtype=torch.float32)
+    x, logits, grad = tokens_for(0, 6, 4, 2, 16, torch.float32)
+    ids, w = ex.route(logits, 2)
+    rows = exchange.dispatch(x, ids)
+    out = exchange.combine(rows * 2, w)
+    want = exchange.combine_backward(grad, w)[1]
+    with pytest.raises(RuntimeFailure):
+        exchange.dispatch(x, ids[:5])                             # choices of fewer tokens
+    assert torch.equal(exchange.combine_backward(grad, w)[1], want)
+    assert torch.equal(exchange.combine(rows * 2, w), out)
+    with pytest.raises(RuntimeFailure):
+        exchange.combine(rows * 3, w[:5])
+    with pytest.raises(RuntimeFailure, match="combine"):          # that combine did not finish, and its rows are gone
+        exchange.combine_backward(grad, w)

@@ -100,8 +100,9 @@ class ExpertExchange:
         self._check_tokens(x, "x")
         if self.comm.world > 1 and self.capacity > 1 << 24:
             raise RuntimeFailure("a capacity above 2^24 cannot be exchanged")
-        self.order, self._returned = ops.sort_by_expert(ids, self.experts, capacity=self.capacity), None
-        rows = ops.dispatch(x.detach(), self.order, out=self._buffer("sent"))
+        order = ops.sort_by_expert(ids, self.experts, capacity=self.capacity)
+        rows = ops.dispatch(x.detach(), order, out=self._buffer("sent"))
+        self.order, self._returned = order, None
         self.counts = self._exchange_counts(self.order.counts)
         return self._exchange(rows, "received")
 
@@ -116,9 +117,11 @@ class ExpertExchange:
         """``out`` [tokens, hidden]: the experts' rows back at their tokens, weighted with ``weights`` and summed."""
         order = self._dispatched()
         self._check_rows(rows, "rows")
+        self._returned = None
         back = self._exchange(rows.detach(), "returned")
+        out = ops.combine(back, weights.detach(), order)
         self._returned = back
-        return ops.combine(back, weights.detach(), order)
+        return out
 
     def combine_backward(self, grad_out: torch.Tensor, weights: torch.Tensor):
         """``(grad_rows, grad_weights)`` of the last :meth:`combine`: the gradient of this rank's expert rows and of
