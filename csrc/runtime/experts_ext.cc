@@ -100,7 +100,9 @@ ExchangeRowsArgs row_args(const Tensor& in, const Tensor& out, const Tensor& slo
   return a;
 }
 
-// the result [rows, columns] of `like`'s dtype: a new tensor, or `out` if it is one of that kind, away from `like`
+// The result [rows, columns] of `like`'s dtype: a new tensor, or `out` if it is one of that kind, away from `like`.
+// A write into `out` counts as an in-place change, so that a graph that has saved it sees it (tensors of inference
+// mode have no versions, and no graph can have saved them).
 Tensor made(const std::optional<Tensor>& out, int64_t rows, int64_t columns, const Tensor& like) {
   if (!out) return empty({rows, columns}, like.scalar_type(), like);
   check_matrix(*out, like, "out");
@@ -108,6 +110,8 @@ Tensor made(const std::optional<Tensor>& out, int64_t rows, int64_t columns, con
               "out has another shape or dtype than the result");
   TORCH_CHECK(rows <= 1 || out->stride(0) >= columns, "out's rows overlap");
   check_apart(*out, like);
+  TORCH_CHECK(!(out->requires_grad() && at::GradMode::is_enabled()), "out requires a gradient");
+  if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
   return *out;
 }
 
@@ -203,14 +207,14 @@ Tensor combine(const Tensor& rows, const std::optional<Tensor>& weights, const T
   check_matrix(rows, rows, "rows");
   check_order(slot, source, rows);
   TORCH_CHECK(rows.size(0) == source.numel(), "rows has another number of rows than the order");
-  c10::cuda::CUDAGuard guard(rows.device());
-  auto tokens = made(out, slot.size(0), rows.size(1), rows);
-  auto a = row_args(rows, tokens, slot, source);
   if (weights) {
     check_table(*weights, rows, at::kFloat, "weights");
     TORCH_CHECK(weights->sizes() == slot.sizes(), "weights are [tokens, k]");
-    a.weights = weights->data_ptr<float>();
   }
+  c10::cuda::CUDAGuard guard(rows.device());
+  auto tokens = made(out, slot.size(0), rows.size(1), rows);
+  auto a = row_args(rows, tokens, slot, source);
+  if (weights) a.weights = weights->data_ptr<float>();
   done(launch_combine(a, stream()), "combine launch");
   return tokens;
 }
@@ -225,8 +229,8 @@ py::tuple combine_backward(const Tensor& grad, const Tensor& rows, const Tensor&
               rows.scalar_type() == grad.scalar_type() && weights.sizes() == slot.sizes(),
               "grad_out, rows, weights and the order do not fit together");
   c10::cuda::CUDAGuard guard(grad.device());
-  auto grad_rows = made(out, source.numel(), grad.size(1), grad);
   if (out) check_apart(*out, rows);
+  auto grad_rows = made(out, source.numel(), grad.size(1), grad);
   auto grad_weights = empty(slot.sizes(), at::kFloat, grad);
   auto a = row_args(grad, grad_rows, slot, source);
   a.saved = rows.data_ptr();

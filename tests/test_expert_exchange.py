@@ -257,3 +257,47 @@ def test_a_refused_call_leaves_the_exchange_as_it_was():
         exchange.combine(rows * 3, w[:5])
     with pytest.raises(RuntimeFailure, match="combine"):          # that combine did not finish, and its rows are gone
         exchange.combine_backward(grad, w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("world", [1, 2])
+def test_autograd_sees_that_rows_were_overwritten(world):
+    """Rows that a learnable expert's graph has saved: its backward pass works until the next dispatch overwrites them."""
+    gpu()
+    links, errors = Threads(world), []
+
+    def rank_main(rank):
+        try:
+            engine = links.engine(rank)
+            copy = engine.all_to_all
+            engine.all_to_all = lambda inp, out: copy(inp, out.data)          # as a kernel writes: unseen by autograd
+            exchange = ExpertExchange(engine, experts=4, hidden=16, capacity=8, dtype=torch.float32)
+            x, logits, grad = tokens_for(rank, 6, 4, 2, 16, torch.float32)
+            ids, w = ex.route(logits, 2)
+            expert = torch.ones(16, device="cuda", requires_grad=True)
+            rows = exchange.dispatch(x, ids)
+            y = rows * expert
+            exchange.combine(y, w)
+            grad_rows, _ = exchange.combine_backward(grad, w)
+            exchange.dispatch_backward(grad_rows)
+            parts = grad_rows.double() * rows.double()
+            y.backward(grad_rows)
+            # products and sums of the rows: as many roundings as there are rows, and one for the product
+            bound = (rows.size(0) + 1) * 2.0 ** -24 * parts.abs().sum(0)
+            assert bool(((expert.grad.double() - parts.sum(0)).abs() <= bound).all())
+            y = exchange.dispatch(x, ids) * expert
+            z = exchange.combine(y, w) * expert                   # rows that came back to the tokens
+            exchange.dispatch(x, ids)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward(grad_rows)
+            z.backward(grad)
+        except BaseException as error:                           # noqa: BLE001  (reported by the test; pytest's own too)
+            errors.append(error)
+            links.gate.abort()
+
+    threads = [threading.Thread(target=rank_main, args=(r,)) for r in range(world)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors

@@ -811,3 +811,50 @@ def test_quantize_int4_keeps_groups_whose_scale_underflows(dtype, scale_dtype):
     back = dequantized(packed, scales, 32)
     assert bool(((back - w.double()).abs() <= least * 0.5).all())
     assert bool((back[2] == 0).all()) and back[1, 3] == least
+
+
+def calls_with_out(g, device="cuda"):
+    """Each call that takes ``out``, as (call of out, the shape of out), on small inputs of bfloat16."""
+    i32 = dict(dtype=torch.int32, device=device)
+    order = ex.ExpertOrder(torch.tensor([[0, 2], [1, 3], [4, 5]], **i32), torch.tensor([0, 2, 1, 3, 4, 5], **i32),
+                           torch.tensor([6], **i32), torch.tensor([0], **i32))
+    x, rows = (torch.randn(n, 32, generator=g, device=device).bfloat16() for n in (3, 6))
+    w = torch.rand(3, 2, generator=g, device=device)
+    packed = torch.zeros(1, 5, 16, dtype=torch.uint8, device=device)
+    scales = torch.ones(1, 5, 1, dtype=torch.bfloat16, device=device)
+    return [(lambda out: ex.dispatch(x, order, out=out), (6, 32)),
+            (lambda out: ex.dispatch_backward(rows, order, out=out), (3, 32)),
+            (lambda out: ex.combine(rows, w, order, out=out), (3, 32)),
+            (lambda out: ex.combine_backward(x, rows, w, order, out=out), (6, 32)),
+            (lambda out: ex.expert_matmul_int4(rows, order.starts, order.counts, packed, scales, out=out), (6, 5))]
+
+
+def test_an_out_that_requires_a_gradient_is_refused():
+    for call, shape in calls_with_out(torch.Generator().manual_seed(1), "cpu"):
+        with pytest.raises(RuntimeFailure, match="gradient"):
+            call(torch.zeros(shape, dtype=torch.bfloat16, requires_grad=True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(5))
+def test_autograd_sees_writes_into_out(which):
+    """A buffer that a graph has saved and that a call overwrites stops that graph's backward pass, as torch's own
+    ``out=`` does; a slice of it too."""
+    g = cuda(71)
+    call, shape = calls_with_out(g)[which]
+    wide = torch.zeros(shape[0], shape[1] + 8, dtype=torch.bfloat16, device="cuda")
+    leaf = torch.ones_like(wide, requires_grad=True)
+    loss = (leaf * wide).sum()
+    call(wide[:, 8:])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    held = torch.zeros(shape, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeFailure, match="gradient"):
+        call(held)
+    with torch.no_grad():
+        call(held)
+    with torch.inference_mode():
+        kept = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+        call(kept)
+    call(kept)                                                    # it has no versions, and no graph can have saved it
+    assert torch.equal(kept, held)

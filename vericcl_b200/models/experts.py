@@ -25,8 +25,8 @@ class ExpertExchange:
 
     Rows are ordered by (source rank, local expert, place); ``starts`` and ``counts`` say which of them hold tokens,
     the others are zero.  Rows that a call returns are the exchange's own buffers: they hold until the same call of
-    this object runs again, so a layer whose backward pass is still to come keeps its own exchange.  Calls run on the
-    current stream, in the same order on every rank.
+    this object runs again, so a layer whose backward pass is still to come keeps its own exchange (autograd refuses a
+    graph whose saved rows were overwritten).  Calls run on the current stream, in the same order on every rank.
     """
 
     def __init__(self, engine, *, experts: int, hidden: int, capacity: int, dtype: torch.dtype = torch.bfloat16):
@@ -76,6 +76,7 @@ class ExpertExchange:
             return rows
         out = self._buffer(name)
         self.engine.all_to_all(rows, out)
+        torch.autograd.graph.increment_version(out)               # a graph that has saved these rows sees the write
         return out
 
     def _exchange_counts(self, counts: torch.Tensor) -> torch.Tensor:

@@ -14,7 +14,8 @@ the form to capture: autograd refuses under capture, because the accumulation in
 still holds would run on a stream outside the capture.
 
 Matrices are ``[rows, hidden]`` with contiguous rows at any row stride (a column slice of a wider matrix, a row
-broadcast by ``expand``); ``out`` may be such a view too, must not overlap an input and is written whole.
+broadcast by ``expand``); ``out`` may be such a view too, must not overlap an input and is written whole, which
+autograd sees as an in-place change of it.
 :class:`~vericcl_b200.models.ExpertExchange` puts these around an engine's AllToAll.
 """
 from __future__ import annotations
@@ -110,7 +111,8 @@ def _on_gpu(first, *others):
 
 
 def _result(out, rows, like, name, columns=None):
-    """Refuse an ``out`` that is not the result's shape and dtype or whose rows overlap each other or an input."""
+    """Refuse an ``out`` that is not the result's shape and dtype, whose rows overlap each other, or that autograd
+    follows."""
     if out is None:
         return
     columns = like.size(1) if columns is None else columns
@@ -118,6 +120,8 @@ def _result(out, rows, like, name, columns=None):
         raise RuntimeFailure("%s must be [%d, %d] of %s" % (name, rows, columns, like.dtype))
     if (columns > 1 and out.stride(1) != 1) or (rows > 1 and out.stride(0) < columns):
         raise RuntimeFailure("%s must have contiguous rows that do not overlap" % name)
+    if out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeFailure("%s requires a gradient, which a call that writes into it would lose" % name)
 
 
 def _span(t):
