@@ -554,8 +554,10 @@ cudaError_t launch_group(const Int4Args& a, cudaStream_t stream) {
 
 }  // namespace
 
+// The device is waited for: a copy on the legacy default stream alone does not wait for non-blocking streams.
 cudaError_t int4_late_copies(int* flag) {
-  cudaError_t e = cudaMemcpyFromSymbol(flag, late_copies, sizeof(int));
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(flag, late_copies, sizeof(int));
   const int none = 0;
   if (e == cudaSuccess && *flag) e = cudaMemcpyToSymbol(late_copies, &none, sizeof(int));
   return e;

@@ -224,6 +224,7 @@ struct Int4Args {
   long long out_stride;
 };
 cudaError_t launch_int4_product(const Int4Args& args, cudaStream_t stream);
-cudaError_t int4_late_copies(int* flag);   // 1 if a copy of a product did not arrive in time since the last call
+// Waits for the current device; 1 if a copy of one of its products did not arrive in time since the last call.
+cudaError_t int4_late_copies(int* flag);
 
 }  // namespace vb

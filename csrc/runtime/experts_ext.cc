@@ -297,6 +297,7 @@ void bind_experts(py::module_& m) {
   m.def("combine_backward", &combine_backward);
   m.def("int4_product", &int4_product);
   m.def("int4_late_copies", []() {
+    py::gil_scoped_release release;      // it waits for the GPU
     int flag = 0;
     done(int4_late_copies(&flag), "read the late-copy flag");
     return flag != 0;

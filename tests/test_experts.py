@@ -858,3 +858,34 @@ def test_autograd_sees_writes_into_out(which):
         call(kept)
     call(kept)                                                    # it has no versions, and no graph can have saved it
     assert torch.equal(kept, held)
+
+
+@pytest.mark.gpu
+def test_check_status_waits_for_products_on_any_stream():
+    g = cuda(81)
+    args = product_case(g, 3, 2, 2, 40, 128, 64, torch.bfloat16, torch.bfloat16)
+    a = torch.zeros(8192, 8192, dtype=torch.bfloat16, device="cuda")
+    a @ a
+    ex.expert_matmul_int4(*args)
+    ex.check_status()                                             # whatever is set up once is
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for _ in range(100):                                      # tens of milliseconds before the product starts
+            a = a @ a
+        ex.expert_matmul_int4(*args)
+    ex.check_status()
+    assert stream.query()
+
+
+@pytest.mark.gpu
+def test_check_status_is_refused_under_capture():
+    cuda()
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(8, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        with pytest.raises(RuntimeFailure, match="capture"):
+            ex.check_status()
+    graph.replay()
+    ex.check_status()
+    assert bool((y == 1).all())

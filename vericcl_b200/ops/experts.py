@@ -403,7 +403,10 @@ def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.T
 
 
 def check_status() -> None:
-    """Raise when a 4-bit product on the current GPU gave up waiting for its weights since the last check (it waits
-    for the GPU; not for a stream that is being captured)."""
+    """Raise when a 4-bit product on the current GPU gave up waiting for its weights since the last check.  It waits
+    for all streams of that GPU, so it is refused while the current stream is being captured; other GPUs have their
+    own status."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeFailure("check_status waits for the GPU and cannot be called under graph capture")
     if _mod().int4_late_copies():
         raise RuntimeFailure("a 4-bit product's copy of weights did not arrive in time; its outputs are NaN")
