@@ -222,6 +222,7 @@ struct Int4Args {
   int group, dtype;
   void* out;                 // [rows, n], rows out_stride apart
   long long out_stride;
+  int give_up;               // 1: no tile of weights is waited for, as if none arrived in time (for tests)
 };
 cudaError_t launch_int4_product(const Int4Args& args, cudaStream_t stream);
 // Waits for the current device; 1 if a copy of one of its products did not arrive in time since the last call.

@@ -242,7 +242,7 @@ py::tuple combine_backward(const Tensor& grad, const Tensor& rows, const Tensor&
 }
 
 Tensor int4_product(const Tensor& x, const Tensor& starts, const Tensor& counts, const Tensor& packed,
-                    const Tensor& scales, const std::optional<Tensor>& out) {
+                    const Tensor& scales, const std::optional<Tensor>& out, bool give_up) {
   check_matrix(x, x, "rows");
   check_table(starts, x, at::kInt, "starts");
   check_table(counts, x, at::kInt, "counts");
@@ -280,6 +280,7 @@ Tensor int4_product(const Tensor& x, const Tensor& starts, const Tensor& counts,
   a.dtype = code_of(x);
   a.out = y.data_ptr();
   a.out_stride = y.stride(0);
+  a.give_up = give_up ? 1 : 0;
   done(launch_int4_product(a, stream()), "4-bit product launch");
   return y;
 }

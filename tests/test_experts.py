@@ -889,3 +889,27 @@ def test_check_status_is_refused_under_capture():
     graph.replay()
     ex.check_status()
     assert bool((y == 1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,experts,active,n,inner,group", [(3, 4, 2, 33, 32, 32), (8, 8, 8, 256, 4096, 128),
+                                                               (40, 2, 2, 130, 1600, 64)])
+def test_int4_product_whose_waits_run_out(monkeypatch, rows, experts, active, n, inner, group):
+    """Every wait given up at once (the copies themselves arrive): covered rows are NaN, the others zero, the
+    status is raised once, and the next product is right.  Sizes of one tile, of a cluster and of several tiles."""
+    g = cuda(91)
+    x, starts, counts, packed, scales = product_case(g, rows, experts, active, n, inner, group, torch.bfloat16,
+                                                     torch.bfloat16)
+    x = torch.cat([x, x[:2]])                                     # two rows that no segment covers
+    ex.check_status()
+    with monkeypatch.context() as patch:
+        patch.setattr(ex, "_GIVE_UP", True)
+        late = ex.expert_matmul_int4(x, starts, counts, packed, scales)
+    with pytest.raises(RuntimeFailure, match="in time"):
+        ex.check_status()
+    ex.check_status()
+    assert bool(late[:rows].isnan().all()) and bool((late[rows:] == 0).all())
+    got = ex.expert_matmul_int4(x, starts, counts, packed, scales)
+    want, size = product_reference(x, starts, counts, packed, scales, group)
+    close(got, want, size, torch.bfloat16, 2 * (inner + 3 * inner // group))
+    ex.check_status()

@@ -32,6 +32,7 @@ MAX_COLUMNS = 1 << 22
 INT4_GROUPS = (32, 64, 128)
 _DTYPES = frozenset({torch.float32, torch.bfloat16, torch.float16})
 _INT_MAX = 2 ** 31 - 1
+_GIVE_UP = False             # True: 4-bit products wait for no weights, as if they arrived too late
 
 _module = None
 
@@ -399,7 +400,7 @@ def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.T
     weights did not arrive in a second are NaN, and :func:`check_status` says so.
     """
     return _call("int4_product", lambda: _check_product(rows, starts, counts, packed, scales, out), rows, starts, counts,
-                 packed, scales, out)
+                 packed, scales, out, _GIVE_UP)
 
 
 def check_status() -> None:
