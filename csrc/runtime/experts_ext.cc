@@ -40,16 +40,23 @@ cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 constexpr int64_t kMaxColumns = 1 << 22;
 
+// the kernels carry no forward-mode tangents, and a result without them would read as one that does not change
+void check_tangent(const Tensor& t, const char* name) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), name, " carries a forward-mode gradient");
+}
+
 // a CUDA matrix on `like`'s device whose rows are contiguous
 void check_matrix(const Tensor& t, const Tensor& like, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " is not on the call's GPU");
   TORCH_CHECK(t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && t.size(1) <= kMaxColumns, name,
               " is no matrix of contiguous rows");
+  check_tangent(t, name);
 }
 
 void check_table(const Tensor& t, const Tensor& like, at::ScalarType type, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.is_contiguous() && t.scalar_type() == type, name,
               " is not a contiguous table of its type on the call's GPU");
+  check_tangent(t, name);
 }
 
 // the bytes from a matrix's first element to its last

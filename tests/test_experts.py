@@ -913,3 +913,44 @@ def test_int4_product_whose_waits_run_out(monkeypatch, rows, experts, active, n,
     want, size = product_reference(x, starts, counts, packed, scales, group)
     close(got, want, size, torch.bfloat16, 2 * (inner + 3 * inner // group))
     ex.check_status()
+
+
+def float_calls(g, device):
+    """(call of its float tensors, those tensors) of every operator, on small inputs."""
+    i32 = dict(dtype=torch.int32, device=device)
+    order = ex.ExpertOrder(torch.tensor([[0, 2], [1, 3]], **i32), torch.tensor([0, 2, 1, 3], **i32),
+                           torch.tensor([4], **i32), torch.tensor([0], **i32))
+    draw = lambda *shape: torch.randn(shape, generator=g, device=device)     # noqa: E731
+    ids = torch.tensor([[0, 2], [1, 0]], **i32)
+    packed = torch.zeros(1, 5, 16, dtype=torch.uint8, device=device)
+    return [(lambda l: ex.route(l, 2), [draw(2, 3)]),
+            (lambda l, w, u: ex.route_backward(l, ids, w, u), [draw(2, 3), draw(2, 2), draw(2, 2)]),
+            (lambda x: ex.dispatch(x, order), [draw(2, 8)]),
+            (lambda r: ex.dispatch_backward(r, order), [draw(4, 8)]),
+            (lambda r, w: ex.combine(r, w, order), [draw(4, 8), draw(2, 2)]),
+            (lambda u, r, w: ex.combine_backward(u, r, w, order), [draw(2, 8), draw(4, 8), draw(2, 2)]),
+            (lambda r, s: ex.expert_matmul_int4(r.bfloat16(), order.starts, order.counts, packed, s),
+             [draw(4, 32), draw(1, 5, 1)])]
+
+
+def tangents_are_refused(device):
+    import torch.autograd.forward_ad as fwd
+    for call, inputs in float_calls(torch.Generator(device=device).manual_seed(3), device):
+        for which in range(len(inputs)):
+            with fwd.dual_level():
+                given = list(inputs)
+                given[which] = fwd.make_dual(given[which], torch.ones_like(given[which]))
+                with pytest.raises(RuntimeFailure, match="forward-mode"):
+                    call(*given)
+        if device == "cuda":
+            call(*inputs)
+
+
+def test_forward_mode_tangents_are_refused():
+    tangents_are_refused("cpu")
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused_on_the_gpu():
+    cuda()
+    tangents_are_refused("cuda")

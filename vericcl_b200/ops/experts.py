@@ -11,7 +11,7 @@ All run on the current stream of their tensors' GPU, allocate nothing but their 
 the host and can be captured into a CUDA graph.  ``route``, ``dispatch`` and ``combine`` take part in autograd;
 ``route_backward``, ``dispatch_backward`` and ``combine_backward`` are the same gradients as plain calls, which is
 the form to capture: autograd refuses under capture, because the accumulation into a leaf that an eager graph
-still holds would run on a stream outside the capture.
+still holds would run on a stream outside the capture.  Forward-mode gradients are refused.
 
 Matrices are ``[rows, hidden]`` with contiguous rows at any row stride (a column slice of a wider matrix, a row
 broadcast by ``expand``); ``out`` may be such a view too, must not overlap an input and is written whole, which
@@ -21,6 +21,7 @@ autograd sees as an in-place change of it.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from vericcl_b200.errors import RuntimeFailure
@@ -79,6 +80,11 @@ class ExpertOrder:
 
 # -- checks -----------------------------------------------------------------------------------------------
 
+def _no_tangent(t, name):
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeFailure("%s carries a forward-mode gradient: these operators have reverse-mode gradients only" % name)
+
+
 def _matrix(t, name):
     if t.dim() != 2 or t.dtype not in _DTYPES:
         raise RuntimeFailure("%s must be a [rows, columns] matrix of float32, bfloat16 or float16" % name)
@@ -86,11 +92,13 @@ def _matrix(t, name):
         raise RuntimeFailure("%s has more than %d columns" % (name, MAX_COLUMNS))
     if t.size(1) > 1 and t.stride(1) != 1:
         raise RuntimeFailure("%s must have contiguous rows (stride 1 in the last dimension)" % name)
+    _no_tangent(t, name)
 
 
 def _table(t, shape, dtype, name):
     if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
         raise RuntimeFailure("%s must be a contiguous %s tensor of shape %s" % (name, dtype, list(shape)))
+    _no_tangent(t, name)
 
 
 def _order(order):
@@ -290,11 +298,13 @@ def combine_backward(grad_out, rows, weights, order: ExpertOrder, *, out: torch.
     without one; written to ``out`` where given) and the fp32 products ``<grad_out[t], rows[slot]>``, zero where an
     assignment has no row."""
     def check():
-        _check_dispatch(grad_out, order, out, "grad_out")
+        _order(order)
+        _matrix(grad_out, "grad_out")
         _matrix(rows, "rows")
         if tuple(rows.shape) != (order.source.numel(), grad_out.size(1)) or rows.dtype != grad_out.dtype:
             raise RuntimeFailure("rows must be [%d, %d] of %s" % (order.source.numel(), grad_out.size(1), grad_out.dtype))
         _table(weights, order.slot.shape, torch.float32, "weights")
+        _check_dispatch(grad_out, order, out, "grad_out")
         _on_gpu(grad_out, rows, weights)
         _apart(out, "out", rows)
     return _call("combine_backward", check, grad_out, rows, weights, order.slot, order.source, out)
@@ -371,6 +381,7 @@ def _check_product(rows, starts, counts, packed, scales, out):
         raise RuntimeFailure("scales must be a contiguous tensor [experts, n, inner / group] of the rows' dtype or float32")
     if not scales.size(2) or rows.size(1) % scales.size(2) or rows.size(1) // scales.size(2) not in INT4_GROUPS:
         raise RuntimeFailure("groups of 32, 64 or 128 that divide the inner size")
+    _no_tangent(scales, "scales")
     segments = starts.numel()
     if not 1 <= segments <= MAX_EXPERTS or segments % packed.size(0):
         raise RuntimeFailure("1 to %d segments, a multiple of the experts" % MAX_EXPERTS)
