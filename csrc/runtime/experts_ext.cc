@@ -59,15 +59,20 @@ void check_table(const Tensor& t, const Tensor& like, at::ScalarType type, const
   check_tangent(t, name);
 }
 
-// the bytes from a matrix's first element to its last
+// the bytes from the first element of a matrix, or of a contiguous tensor, to its last
 std::pair<const char*, const char*> span(const Tensor& t) {
   const char* lo = static_cast<const char*>(t.data_ptr());
-  return {lo, t.numel() ? lo + ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size() : lo};
+  if (!t.numel()) return {lo, lo};
+  const int64_t length = t.dim() == 2 ? (t.size(0) - 1) * t.stride(0) + t.size(1) : t.numel();
+  return {lo, lo + length * t.element_size()};
 }
 
 void check_apart(const Tensor& out, const Tensor& in) {
   const auto a = span(out), b = span(in);
   TORCH_CHECK(a.first >= b.second || b.first >= a.second, "out overlaps an input");
+}
+void check_apart(const Tensor& out, const std::optional<Tensor>& in) {
+  if (in) check_apart(out, *in);
 }
 
 Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
@@ -107,16 +112,18 @@ ExchangeRowsArgs row_args(const Tensor& in, const Tensor& out, const Tensor& slo
   return a;
 }
 
-// The result [rows, columns] of `like`'s dtype: a new tensor, or `out` if it is one of that kind, away from `like`.
-// A write into `out` counts as an in-place change, so that a graph that has saved it sees it (tensors of inference
+// The result [rows, columns] of `like`'s dtype: a new tensor, or `out` if it is one of that kind, away from `like` and
+// the other inputs.  A write into `out` counts as an in-place change, so that a graph that has saved it sees it (tensors of inference
 // mode have no versions, and no graph can have saved them).
-Tensor made(const std::optional<Tensor>& out, int64_t rows, int64_t columns, const Tensor& like) {
+template <typename... Inputs>
+Tensor made(const std::optional<Tensor>& out, int64_t rows, int64_t columns, const Tensor& like, const Inputs&... inputs) {
   if (!out) return empty({rows, columns}, like.scalar_type(), like);
   check_matrix(*out, like, "out");
   TORCH_CHECK(out->size(0) == rows && out->size(1) == columns && out->scalar_type() == like.scalar_type(),
               "out has another shape or dtype than the result");
   TORCH_CHECK(rows <= 1 || out->stride(0) >= columns, "out's rows overlap");
   check_apart(*out, like);
+  (check_apart(*out, inputs), ...);
   TORCH_CHECK(!(out->requires_grad() && at::GradMode::is_enabled()), "out requires a gradient");
   if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
   return *out;
@@ -204,7 +211,7 @@ Tensor dispatch(const Tensor& x, const Tensor& slot, const Tensor& source, const
   check_order(slot, source, x);
   TORCH_CHECK(x.size(0) == slot.size(0), "x has another number of tokens than the order");
   c10::cuda::CUDAGuard guard(x.device());
-  auto rows = made(out, source.numel(), x.size(1), x);
+  auto rows = made(out, source.numel(), x.size(1), x, slot, source);
   done(launch_dispatch(row_args(x, rows, slot, source), stream()), "dispatch launch");
   return rows;
 }
@@ -219,7 +226,7 @@ Tensor combine(const Tensor& rows, const std::optional<Tensor>& weights, const T
     TORCH_CHECK(weights->sizes() == slot.sizes(), "weights are [tokens, k]");
   }
   c10::cuda::CUDAGuard guard(rows.device());
-  auto tokens = made(out, slot.size(0), rows.size(1), rows);
+  auto tokens = made(out, slot.size(0), rows.size(1), rows, slot, source, weights);
   auto a = row_args(rows, tokens, slot, source);
   if (weights) a.weights = weights->data_ptr<float>();
   done(launch_combine(a, stream()), "combine launch");
@@ -236,8 +243,7 @@ py::tuple combine_backward(const Tensor& grad, const Tensor& rows, const Tensor&
               rows.scalar_type() == grad.scalar_type() && weights.sizes() == slot.sizes(),
               "grad_out, rows, weights and the order do not fit together");
   c10::cuda::CUDAGuard guard(grad.device());
-  if (out) check_apart(*out, rows);
-  auto grad_rows = made(out, source.numel(), grad.size(1), grad);
+  auto grad_rows = made(out, source.numel(), grad.size(1), grad, rows, weights, slot, source);
   auto grad_weights = empty(slot.sizes(), at::kFloat, grad);
   auto a = row_args(grad, grad_rows, slot, source);
   a.saved = rows.data_ptr();
@@ -269,7 +275,7 @@ Tensor int4_product(const Tensor& x, const Tensor& starts, const Tensor& counts,
   TORCH_CHECK(reinterpret_cast<uintptr_t>(packed.data_ptr()) % 16 == 0, "packed starts on a 16-byte boundary");
   c10::cuda::CUDAGuard guard(x.device());
   TORCH_CHECK(!(x.requires_grad() && at::GradMode::is_enabled()), "4-bit products have no gradient");
-  auto y = made(out, x.size(0), packed.size(1), x);
+  auto y = made(out, x.size(0), packed.size(1), x, starts, counts, packed, scales);
   Int4Args a{};
   a.x = x.data_ptr();
   a.x_stride = x.stride(0);

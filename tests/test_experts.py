@@ -954,3 +954,42 @@ def test_forward_mode_tangents_are_refused():
 def test_forward_mode_tangents_are_refused_on_the_gpu():
     cuda()
     tangents_are_refused("cuda")
+
+
+def overlapping_calls(device):
+    """Calls whose out lies over an input that is not the matrix the rows come from."""
+    i32 = dict(dtype=torch.int32, device=device)
+    pool = torch.zeros(4096, device=device)                       # every tensor is a part of it
+    order = ex.ExpertOrder(pool[:8].view(torch.int32).view(4, 2), pool[8:16].view(torch.int32), torch.tensor([8], **i32),
+                           torch.tensor([0], **i32))
+    w, x, rows = pool[16:24].view(4, 2), pool[64:96].view(4, 8), pool[128:192].view(8, 8)
+    elsewhere = pool[1024:1056].view(4, 8)
+    half = pool.view(torch.bfloat16)                              # element 2 i is at pool[i]
+    r16 = half[4096:4096 + 8 * 32].view(8, 32)
+    packed = pool[512:512 + 20].view(torch.uint8).view(1, 5, 16)
+    scales, starts, counts = half[1200:1205].view(1, 5, 1), pool[700:701].view(torch.int32), pool[704:705].view(torch.int32)
+
+    def product(at):
+        return lambda: ex.expert_matmul_int4(r16, starts, counts, packed, scales, out=half[at:at + 40].view(8, 5))
+    return [lambda: ex.dispatch(x, order, out=pool[4:68].view(8, 8)),               # slot
+            lambda: ex.dispatch(elsewhere, order, out=pool[15:79].view(8, 8)),      # source
+            lambda: ex.dispatch_backward(rows, order, out=pool[15:47].view(4, 8)),
+            lambda: ex.combine(rows, w, order, out=pool[7:39].view(4, 8)),
+            lambda: ex.combine(rows, w, order, out=pool[23:55].view(4, 8)),         # weights
+            lambda: ex.combine_backward(elsewhere, rows, w, order, out=pool[23:87].view(8, 8)),
+            lambda: ex.combine_backward(elsewhere, rows, w, order, out=pool[100:164].view(8, 8)),
+            product(2 * 512 - 39), product(2 * 512 + 39), product(1204), product(1200 - 39), product(1400), product(1409)]
+
+
+def test_an_out_over_any_input_is_refused():
+    for i, call in enumerate(overlapping_calls("cpu")):
+        with pytest.raises(RuntimeFailure, match="overlaps"):
+            call()
+
+
+@pytest.mark.gpu
+def test_an_out_over_any_input_is_refused_on_the_gpu():
+    cuda()
+    for call in overlapping_calls("cuda"):
+        with pytest.raises(RuntimeFailure, match="overlaps"):
+            call()

@@ -134,16 +134,19 @@ def _result(out, rows, like, name, columns=None):
 
 
 def _span(t):
+    """The bytes from the first element of a matrix, or of a contiguous tensor, to its last."""
     lo = t.data_ptr()
-    return lo, lo + ((t.size(0) - 1) * t.stride(0) + t.size(1)) * t.element_size() if t.numel() else lo
+    if not t.numel():
+        return lo, lo
+    length = (t.size(0) - 1) * t.stride(0) + t.size(1) if t.dim() == 2 else t.numel()
+    return lo, lo + length * t.element_size()
 
 
 def _apart(out, name, *inputs):
     if out is None or not out.numel():
         return
     lo, hi = _span(out)
-    for t in inputs:
-        a, b = _span(t)
+    for a, b in (_span(t) for t in inputs if t is not None):
         if a < hi and lo < b:
             raise RuntimeFailure("%s overlaps an input" % name)
 
@@ -252,8 +255,8 @@ def _check_dispatch(x, order, out, name):
     if x.size(0) != slot.size(0):
         raise RuntimeFailure("%s has %d tokens, the order %d" % (name, x.size(0), slot.size(0)))
     _result(out, source.numel(), x, "out")
+    _apart(out, "out", x, slot, source)
     _on_gpu(x, slot, source, out)
-    _apart(out, "out", x)
 
 
 def _check_combine(rows, weights, order, out, name):
@@ -264,8 +267,8 @@ def _check_combine(rows, weights, order, out, name):
     if weights is not None:
         _table(weights, slot.shape, torch.float32, "weights")
     _result(out, slot.size(0), rows, "out")
+    _apart(out, "out", rows, slot, source, weights)
     _on_gpu(rows, slot, source, weights, out)
-    _apart(out, "out", rows)
 
 
 def dispatch(x: torch.Tensor, order: ExpertOrder, *, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -304,9 +307,9 @@ def combine_backward(grad_out, rows, weights, order: ExpertOrder, *, out: torch.
         if tuple(rows.shape) != (order.source.numel(), grad_out.size(1)) or rows.dtype != grad_out.dtype:
             raise RuntimeFailure("rows must be [%d, %d] of %s" % (order.source.numel(), grad_out.size(1), grad_out.dtype))
         _table(weights, order.slot.shape, torch.float32, "weights")
+        _apart(out, "out", rows, weights)
         _check_dispatch(grad_out, order, out, "grad_out")
         _on_gpu(grad_out, rows, weights)
-        _apart(out, "out", rows)
     return _call("combine_backward", check, grad_out, rows, weights, order.slot, order.source, out)
 
 
@@ -394,8 +397,8 @@ def _check_product(rows, starts, counts, packed, scales, out):
     if rows.requires_grad and torch.is_grad_enabled():
         raise RuntimeFailure("4-bit products have no gradient: detach the rows")
     _result(out, rows.size(0), rows, "out", packed.size(1))
+    _apart(out, "out", rows, starts, counts, packed, scales)
     _on_gpu(rows, starts, counts, packed, scales, out)
-    _apart(out, "out", rows)
 
 
 def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, packed: torch.Tensor,
