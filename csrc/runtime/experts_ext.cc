@@ -59,17 +59,30 @@ void check_table(const Tensor& t, const Tensor& like, at::ScalarType type, const
   check_tangent(t, name);
 }
 
-// the bytes from the first element of a matrix, or of a contiguous tensor, to its last
-std::pair<const char*, const char*> span(const Tensor& t) {
-  const char* lo = static_cast<const char*>(t.data_ptr());
-  if (!t.numel()) return {lo, lo};
-  const int64_t length = t.dim() == 2 ? (t.size(0) - 1) * t.stride(0) + t.size(1) : t.numel();
-  return {lo, lo + length * t.element_size()};
+// A matrix in memory, in bytes; a contiguous tensor of other dimensions is one row.
+struct Extent {
+  int64_t lo, width, pitch, rows;
+};
+Extent extent(const Tensor& t) {
+  const int64_t lo = (int64_t)reinterpret_cast<uintptr_t>(t.data_ptr()), size = t.element_size();
+  if (!t.numel()) return {lo, 0, 0, 0};
+  if (t.dim() != 2) return {lo, t.numel() * size, 0, 1};
+  return {lo, t.size(1) * size, t.stride(0) * size, t.size(0)};
+}
+
+// Column ranges of one matrix lie in one span of memory without meeting: with one pitch, what counts is the distance
+// of the first columns within it.  Different pitches are compared by their spans.
+bool apart(const Extent& a, const Extent& b) {
+  if (!a.rows || !b.rows) return true;
+  if (a.lo + (a.rows - 1) * a.pitch + a.width <= b.lo || b.lo + (b.rows - 1) * b.pitch + b.width <= a.lo) return true;
+  const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+  if ((b.rows > 1 && b.pitch != pitch) || (a.rows == 1 && b.rows == 1) || pitch < a.width || pitch < b.width) return false;
+  const int64_t between = ((b.lo - a.lo) % pitch + pitch) % pitch;
+  return between >= a.width && between + b.width <= pitch;
 }
 
 void check_apart(const Tensor& out, const Tensor& in) {
-  const auto a = span(out), b = span(in);
-  TORCH_CHECK(a.first >= b.second || b.first >= a.second, "out overlaps an input");
+  TORCH_CHECK(apart(extent(out), extent(in)), "out overlaps an input");
 }
 void check_apart(const Tensor& out, const std::optional<Tensor>& in) {
   if (in) check_apart(out, *in);

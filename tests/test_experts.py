@@ -993,3 +993,55 @@ def test_an_out_over_any_input_is_refused_on_the_gpu():
     for call in overlapping_calls("cuda"):
         with pytest.raises(RuntimeFailure, match="overlaps"):
             call()
+
+
+def beside(device):
+    """One matrix whose column ranges are the tokens, the rows and the results."""
+    i32 = dict(dtype=torch.int32, device=device)
+    order = ex.ExpertOrder(torch.tensor([[0, 2], [1, 3]], **i32), torch.tensor([0, 2, 1, 3], **i32),
+                           torch.tensor([4], **i32), torch.tensor([0], **i32))
+    wide = torch.arange(4 * 24, dtype=torch.float32, device=device).view(4, 24)
+    return wide, order, torch.tensor([[1.0, 2], [0.5, 1]], device=device)
+
+
+def test_columns_that_meet_are_refused():
+    wide, order, w = beside("cpu")
+    for call in (lambda: ex.dispatch(wide[:2, :8], order, out=wide[:, 7:15]),
+                 lambda: ex.dispatch(wide[:2, 8:16], order, out=wide[:, 1:9]),
+                 lambda: ex.dispatch(wide[:2, :8], order, out=wide[:, :8]),
+                 lambda: ex.dispatch(wide.view(8, 12)[:2, :6], order, out=wide[:, 6:12]),     # other strides
+                 lambda: ex.dispatch_backward(wide[:1, :8].expand(4, 8), order, out=wide[:2, 4:12]),
+                 lambda: ex.combine(wide[:, 8:16], w, order, out=wide[:2, 15:23]),
+                 # the last column of a row and the first of the next
+                 lambda: ex.combine(wide[:, :8], w, order, out=wide.view(-1)[17:17 + 48].view(2, 24)[:, :8])):
+        with pytest.raises(RuntimeFailure, match="overlaps"):
+            call()
+
+
+def test_columns_beside_each_other_are_not_an_overlap():
+    wide, order, w = beside("cpu")
+    for call in (lambda: ex.dispatch(wide[:2, :8], order, out=wide[:, 8:16]),
+                 lambda: ex.dispatch(wide[1:3, 16:], order, out=wide[:, 8:16]),
+                 lambda: ex.combine(wide[:, 8:16], w, order, out=wide[:2, 16:24]),
+                 lambda: ex.combine(wide[:, :8], w, order, out=wide.view(-1)[16:16 + 48].view(2, 24)[:, :8]),
+                 lambda: ex.combine_backward(wide[:2, 16:], wide[:, :8], w, order, out=wide[:, 8:16])):
+        with pytest.raises(RuntimeFailure, match="CUDA"):         # nothing else is wrong with them
+            call()
+
+
+@pytest.mark.gpu
+def test_columns_of_one_matrix_as_inputs_and_out():
+    cuda()
+    wide, order, w = beside("cuda")
+    start = wide.clone()
+    rows = ex.dispatch(wide[:2, :8], order, out=wide[:, 8:16])
+    assert torch.equal(rows, start[[0, 1, 0, 1], :8])
+    assert torch.equal(wide[:, :8], start[:, :8]) and torch.equal(wide[:, 16:], start[:, 16:])
+    ex.combine(wide[:, 8:16], w, order, out=wide[1:3, 16:])
+    assert torch.equal(wide[1:3, 16:], start[:2, :8] * torch.tensor([[3.0], [1.5]], device="cuda"))
+    grad, got_w = ex.combine_backward(wide[1:3, 16:], wide[:, 8:16], w, order, out=wide[:, :8])
+    up = wide[1:3, 16:]
+    assert torch.equal(grad, up.repeat(2, 1) * torch.tensor([[1.0], [0.5], [2], [1]], device="cuda"))
+    assert torch.allclose(got_w, (up * wide[:2, 8:16]).sum(1, keepdim=True).expand(2, 2))
+    with pytest.raises(RuntimeFailure, match="overlaps"):
+        ex.dispatch(wide[:2, :8], order, out=wide[:, 7:15])

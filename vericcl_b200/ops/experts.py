@@ -14,8 +14,8 @@ the form to capture: autograd refuses under capture, because the accumulation in
 still holds would run on a stream outside the capture.  Forward-mode gradients are refused.
 
 Matrices are ``[rows, hidden]`` with contiguous rows at any row stride (a column slice of a wider matrix, a row
-broadcast by ``expand``); ``out`` may be such a view too, must not overlap an input and is written whole, which
-autograd sees as an in-place change of it.
+broadcast by ``expand``); ``out`` may be such a view too, must not overlap an input (columns of one matrix beside each
+other do not) and is written whole, which autograd sees as an in-place change of it.
 :class:`~vericcl_b200.models.ExpertExchange` puts these around an engine's AllToAll.
 """
 from __future__ import annotations
@@ -133,22 +133,35 @@ def _result(out, rows, like, name, columns=None):
         raise RuntimeFailure("%s requires a gradient, which a call that writes into it would lose" % name)
 
 
-def _span(t):
-    """The bytes from the first element of a matrix, or of a contiguous tensor, to its last."""
-    lo = t.data_ptr()
+def _extent(t):
+    """``(address, bytes of a row, bytes between rows, rows)``; a contiguous tensor of other dimensions is one row."""
+    size = t.element_size()
     if not t.numel():
-        return lo, lo
-    length = (t.size(0) - 1) * t.stride(0) + t.size(1) if t.dim() == 2 else t.numel()
-    return lo, lo + length * t.element_size()
+        return t.data_ptr(), 0, 0, 0
+    if t.dim() != 2:
+        return t.data_ptr(), t.numel() * size, 0, 1
+    return t.data_ptr(), t.size(1) * size, t.stride(0) * size, t.size(0)
+
+
+def _meet(a, b) -> bool:
+    """Whether two extents may share a byte.  Column ranges of one matrix lie in one span of memory without meeting:
+    with one pitch, what counts is the distance of the first columns within it.  Different pitches are compared by
+    their spans."""
+    (a_lo, a_width, a_pitch, a_rows), (b_lo, b_width, b_pitch, b_rows) = a, b
+    if not a_rows or not b_rows:
+        return False
+    if a_lo + (a_rows - 1) * a_pitch + a_width <= b_lo or b_lo + (b_rows - 1) * b_pitch + b_width <= a_lo:
+        return False
+    pitch = a_pitch if a_rows > 1 else b_pitch
+    if (b_rows > 1 and b_pitch != pitch) or a_rows == b_rows == 1 or pitch < max(a_width, b_width):
+        return True
+    between = (b_lo - a_lo) % pitch
+    return between < a_width or between + b_width > pitch
 
 
 def _apart(out, name, *inputs):
-    if out is None or not out.numel():
-        return
-    lo, hi = _span(out)
-    for a, b in (_span(t) for t in inputs if t is not None):
-        if a < hi and lo < b:
-            raise RuntimeFailure("%s overlaps an input" % name)
+    if out is not None and any(_meet(_extent(out), _extent(t)) for t in inputs if t is not None):
+        raise RuntimeFailure("%s overlaps an input" % name)
 
 
 def _learns() -> bool:
