@@ -230,6 +230,9 @@ __device__ __forceinline__ void group_product(float (&acc)[COLS][4], const unsig
   }
 }
 
+// items of more than 8 rows of a segment; its length rounded up may pass 31 bits
+__device__ __forceinline__ int longer_items(int rows) { return (int)(((unsigned)rows + kItem - 9) / kItem); }
+
 struct Geometry {
   long long slice;     // inner values of one CTA of the cluster, whole tiles
   int aligned;         // rows of x can be read 16 bytes at a time
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_
       const long long lo = first[i], hi = min(lo + count[i], a.rows);
       first[i] = max(first[i], 0);
       count[i] = (int)max(hi - first[i], 0ll);
-      mine.x += (count[i] + kItem - 9) / kItem;
+      mine.x += longer_items(count[i]);
       mine.y += (unsigned)(count[i] - 1) % kItem < 8 && count[i];
       rows += count[i];
     }
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 2) int4_product_kernel(const __grid_
     }
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int longer = (count[i] + kItem - 9) / kItem, shorter = (unsigned)(count[i] - 1) % kItem < 8 && count[i];
+      const int longer = longer_items(count[i]), shorter = (unsigned)(count[i] - 1) % kItem < 8 && count[i];
       int at = -1;
       if (item >= before && item < before + longer) at = (item - before) * kItem;
       if (shorter && item == before_short) at = longer * kItem;

@@ -1045,3 +1045,20 @@ def test_columns_of_one_matrix_as_inputs_and_out():
     assert torch.allclose(got_w, (up * wide[:2, 8:16]).sum(1, keepdim=True).expand(2, 2))
     with pytest.raises(RuntimeFailure, match="overlaps"):
         ex.dispatch(wide[:2, :8], order, out=wide[:, 7:15])
+
+
+@pytest.mark.gpu
+def test_int4_product_of_the_longest_segment():
+    """One segment of 2^31 - 1 rows (one row repeated): its length rounded up to whole items passes 31 bits."""
+    g = cuda(101)
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    rows, i32 = 2 ** 31 - 1, dict(dtype=torch.int32, device="cuda")
+    x = normal(g, 1, 32, dtype=torch.bfloat16)
+    packed = torch.randint(0, 256, (1, 1, 16), dtype=torch.uint8, device="cuda", generator=g)
+    scales = torch.ones(1, 1, 1, dtype=torch.bfloat16, device="cuda")
+    one = ex.expert_matmul_int4(x, torch.zeros(1, **i32), torch.ones(1, **i32), packed, scales)
+    assert one[0, 0] != 0 and one[0, 0].isfinite()
+    out = torch.zeros(rows, 1, dtype=torch.bfloat16, device="cuda")
+    ex.expert_matmul_int4(x.expand(rows, 32), torch.zeros(1, **i32), torch.full((1,), rows, **i32), packed, scales, out=out)
+    assert all(bool((part == one[0, 0]).all()) for part in out.split(1 << 28))
