@@ -1062,3 +1062,138 @@ def test_int4_product_of_the_longest_segment():
     out = torch.zeros(rows, 1, dtype=torch.bfloat16, device="cuda")
     ex.expert_matmul_int4(x.expand(rows, 32), torch.zeros(1, **i32), torch.full((1,), rows, **i32), packed, scales, out=out)
     assert all(bool((part == one[0, 0]).all()) for part in out.split(1 << 28))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("experts,k", [(96, 6), (128, 8), (300, 16), (1000, 32)])
+def test_route_masks_nan_and_infinity_among_many_experts(dtype, renormalize, experts, k):
+    """The paths of more than 64 experts: few finite logits, none, the type's lowest value, NaN and +inf."""
+    g = cuda(experts + k)
+    logits = normal(g, 60, experts, dtype=dtype, scale=3.0)
+    scattered = torch.rand(60, experts, device="cuda", generator=g)
+    for t, finite in enumerate([0, 1, k - 1, k, k + 1, 33, 64]):  # so many experts are left, anywhere
+        logits[t].masked_fill_(scattered[t].argsort().argsort() >= finite, -math.inf)
+    logits[10:20].masked_fill_(scattered[10:20] < 0.5, -math.inf)
+    low = torch.finfo(dtype).min
+    logits[20] = low
+    logits[21:25].masked_fill_(scattered[21:25] < 0.9, low)
+    logits[25, 1:] = low
+    finite_rows = list(range(30))
+    logits[30:35, 7] = math.nan
+    logits[35] = math.nan
+    logits[36] = -math.inf
+    logits[36, 70] = math.nan
+    logits[40:45, 90] = math.inf
+    logits[45:48] = math.inf
+    logits[48, 3], logits[48, 88] = math.inf, math.nan
+    spoiled = list(range(30, 36)) + list(range(40, 49))
+    finite_rows += [t for t in range(30, 60) if t not in spoiled]  # 36, a token without a choice, has weights of 0
+    ids, w = ex.route(logits, k, renormalize=renormalize)
+    want_ids, want = reference_route(logits, k, renormalize)
+    assert torch.equal(ids, want_ids)
+    fine = torch.tensor(finite_rows, device="cuda")
+    bound = route_bound(logits[50:])                              # differences to a masked logit do not reach a weight
+    # exp of a difference beyond the type's finite range is 0 on both sides, or below 2^-126 where a subnormal is cut
+    assert bool(((w[fine].double() - want[fine]).abs() <= bound * want[fine] + 2.0 ** -125).all())
+    assert bool(w[spoiled][ids[spoiled] >= 0].isnan().all()) and bool((w[ids < 0] == 0).all())
+    up = normal(g, 60, k)
+    got = ex.route_backward(logits, ids, w, up, renormalize=renormalize)
+    up64 = torch.where(ids >= 0, up.double(), 0.0)
+    inner = (want * up64).sum(1, keepdim=True)
+    expect = torch.zeros(60, experts + 1, dtype=torch.float64, device="cuda")
+    spot = torch.where(ids >= 0, ids.long(), experts)             # a column for what is not chosen
+    if renormalize:
+        expect.scatter_(1, spot, want * (up64 - inner))
+        expect, share = expect[:, :experts], 1.0
+    else:
+        share = torch.softmax(logits.double(), 1).nan_to_num()
+        expect = share * (expect.scatter_(1, spot, up64)[:, :experts] - inner)
+    size = up.abs().max().item() * 2
+    limit = half_step(dtype) * expect.abs() + (4 * bound + 40 * 2.0 ** -24) * size * share + \
+        torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps + 2.0 ** -124
+    rows = [t for t in finite_rows if t != 36]
+    assert bool(((got.double() - expect).abs() <= limit)[rows].all())
+    for t in spoiled:                                             # the chosen experts' gradients are spoiled, or all
+        assert bool(got[t][ids[t][ids[t] >= 0].long()].isnan().all())
+        if renormalize:
+            others = torch.ones(experts, dtype=torch.bool, device="cuda")
+            others[ids[t][ids[t] >= 0].long()] = False
+            assert bool((got[t][others] == 0).all())
+        elif bool((ids[t] >= 0).any()):
+            assert bool(got[t].isnan().all())
+
+
+def torch_order(ids, experts, capacity):
+    """``reference_order`` for many assignments."""
+    flat = ids.reshape(-1).long().cpu()
+    key = torch.where((flat >= 0) & (flat < experts), flat, experts)
+    total = torch.bincount(key, minlength=experts + 1)
+    by_expert = torch.sort(key, stable=True).indices
+    place = torch.empty_like(key)
+    place[by_expert] = torch.arange(len(key)) - (total.cumsum(0) - total)[key[by_expert]]
+    starts = torch.arange(experts) * capacity if capacity else (total.cumsum(0) - total)[:experts]
+    kept = (key < experts) & (place < (capacity or len(key)))
+    slot = torch.where(kept, starts[key.clamp(max=experts - 1)] + place, -1)
+    source = torch.full((experts * capacity if capacity else len(key),), -1)
+    source[slot[kept]] = torch.arange(len(key))[kept]
+    counts = total[:experts].clamp(max=capacity or len(key))
+    return [t.int().cuda() for t in (slot.view(ids.shape), source, counts, starts)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("tokens,k,experts,capacity", [(65536, 8, 1024, None), (65536, 8, 1024, 500), (16397, 8, 1023, 3),
+                                                       (300000, 1, 1, 299999), (40000, 4, 2, 90000)])
+def test_sort_across_the_largest_cluster(dtype, tokens, k, experts, capacity):
+    """16 CTAs with the most experts, whose counts take the most shared memory; few experts with long empty parts."""
+    g = cuda(tokens)
+    ids = random_ids(g, tokens, k, experts, dtype)
+    order = ex.sort_by_expert(ids, experts, capacity=capacity)
+    for got, expect in zip((order.slot, order.source, order.counts, order.starts), torch_order(ids, experts, capacity)):
+        assert torch.equal(got, expect)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hidden", [(torch.float32, 1030), (torch.float32, 1028), (torch.float32, 1027),
+                                          (torch.bfloat16, 2052), (torch.float16, 2051), (torch.bfloat16, 1544)])
+def test_rows_beyond_half_the_l2_with_empty_ones(dtype, hidden):
+    """More than 64 MB of rows, a third of them without a token, in vectors of 16, 8, 4 and 2 bytes."""
+    test_dispatch_and_combine_match_reference(dtype, 6000, 3, 40, 600, hidden)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_int4_product_of_the_smallest_and_largest_rows(dtype, group):
+    """Rows whose products are subnormal in fp32 for bf16 rows (fp16's smallest are not), and rows near the type's largest
+    value with scales that bring the sum back."""
+    g = cuda(group)
+    fine = torch.finfo(dtype)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    inner, n = 4 * group, 21
+    packed = torch.randint(0, 256, (1, n, inner // 2), dtype=torch.uint8, device="cuda", generator=g)
+    signs = torch.randint(0, 2, (3, inner), device="cuda", generator=g) * 2.0 - 1
+    for magnitude, scale in ((fine.smallest_normal, 1.0), (fine.smallest_normal * fine.eps, 1.0),
+                             (fine.smallest_normal, 2.0 ** 14), (fine.max / 2 ** 12, 2.0 ** -14)):
+        x = (signs * magnitude).to(dtype)
+        scales = torch.full((1, n, inner // group), scale, dtype=dtype, device="cuda")
+        args = x, torch.zeros(1, **i32), torch.full((1,), 3, **i32), packed, scales
+        want, size = product_reference(*args, group)
+        close(ex.expert_matmul_int4(*args), want, size, dtype, 2 * (inner + 3 * inner // group))
+
+
+@pytest.mark.gpu
+def test_int4_product_with_overlapping_segments_stays_inside_its_result():
+    """Segments that cover rows twice leave the result undefined, and everything around it as it was."""
+    g = cuda(111)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    _, _, _, packed, scales = product_case(g, 4, 2, 2, 50, 128, 64, torch.bfloat16, torch.bfloat16)
+    x = normal(g, 40, 128, dtype=torch.bfloat16)
+    store = torch.full((42, 60), 7.0, device="cuda", dtype=torch.bfloat16)
+    for starts, counts in (([0, 0, 0, 0], [40, 40, 40, 40]), ([0, 3, 20, 39], [20, 9, 20, 7])):
+        ex.expert_matmul_int4(x, torch.tensor(starts, **i32), torch.tensor(counts, **i32), packed, scales,
+                              out=store[1:41, 5:55])
+        assert bool((store[[0, 41]] == 7).all()) and bool((store[:, :5] == 7).all()) and bool((store[:, 55:] == 7).all())
+    ex.check_status()
