@@ -301,3 +301,27 @@ def test_autograd_sees_that_rows_were_overwritten(world):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+@pytest.mark.gpu
+def test_explicit_gradients_are_handed_on_by_the_caller():
+    """Inputs that require gradients: the exchange records nothing, and its gradients reach the leaves through backward
+    calls of the caller, as autograd's own through the operators do."""
+    gpu()
+    exchange = alone(experts=4, hidden=16, capacity=8, dtype=torch.float32)
+    base, logits, grad = tokens_for(0, 6, 4, 2, 16, torch.float32)
+    x, l = (t.requires_grad_() for t in (base, logits))
+    tokens = x * 3                                                # an activation, no leaf
+    ids, w = ex.route(l, 2)
+    rows = exchange.dispatch(tokens, ids)
+    out = exchange.combine(rows * 2, w)
+    assert w.requires_grad and not rows.requires_grad and not out.requires_grad
+    grad_rows, grad_w = exchange.combine_backward(grad, w)
+    tokens.backward(exchange.dispatch_backward(grad_rows * 2))
+    w.backward(grad_w)
+    x2, l2 = (t.detach().clone().requires_grad_() for t in (x, l))
+    ids2, w2 = ex.route(l2, 2)
+    order = ex.sort_by_expert(ids2, 4, capacity=8)
+    want = ex.combine(ex.dispatch(x2 * 3, order) * 2, w2, order)
+    want.backward(grad)
+    assert torch.equal(out, want) and torch.equal(x.grad, x2.grad) and torch.equal(l.grad, l2.grad)

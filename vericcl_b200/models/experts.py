@@ -3,8 +3,10 @@
 ``ExpertExchange`` puts the operators of :mod:`vericcl_b200.ops.experts` on both sides of
 :meth:`CollectiveEngine.all_to_all`.  Experts are dealt to the ranks in order (rank ``r`` owns ``experts / world``
 of them from ``r * experts / world`` on) and every source rank has ``capacity`` rows at every expert, the equal parts
-an AllToAll exchanges; the rows live in the communicator's heap, so the exchange runs zero-copy.  One rank exchanges
-nothing and uses its rows in place.
+an AllToAll exchanges.  The rows that ``dispatch`` and ``combine_backward`` send and what every exchange receives lie
+in the communicator's heap and need no copy; rows that a caller brings (the experts' results, the gradient of the
+dispatched rows) are first copied to a heap buffer of the engine, unless they lie in the heap themselves
+(``comm.empty``).  One rank exchanges nothing and uses its rows in place.
 """
 from __future__ import annotations
 
@@ -27,6 +29,10 @@ class ExpertExchange:
     the others are zero.  Rows that a call returns are the exchange's own buffers: they hold until the same call of
     this object runs again, so a layer whose backward pass is still to come keeps its own exchange (autograd refuses a
     graph whose saved rows were overwritten).  Calls run on the current stream, in the same order on every rank.
+
+    Autograd stops here: no call records anything, results require no gradient whatever the inputs do, and
+    :meth:`combine_backward` and :meth:`dispatch_backward` are the gradients, to be handed on by the caller
+    (``weights.backward(grad_weights)``, ``x.backward(grad_x)``, or inside a ``torch.autograd.Function``).
     """
 
     def __init__(self, engine, *, experts: int, hidden: int, capacity: int, dtype: torch.dtype = torch.bfloat16):
@@ -148,7 +154,7 @@ class ExpertExchange:
         return grad
 
     def close(self) -> None:
-        """Give the heap buffers back (no exchange may be in flight)."""
+        """Give the exchange's heap buffers back (none may be in flight); the engine keeps its copy buffers."""
         for buf in self._heap.values():
             for t in buf if isinstance(buf, tuple) else (buf,):
                 self.comm.free(t)

@@ -422,9 +422,10 @@ def expert_matmul_int4(rows: torch.Tensor, starts: torch.Tensor, counts: torch.T
     ``rows`` [rows, inner] is bfloat16 or float16; ``starts`` and ``counts`` int32 [segments] (an order's, or one
     segment per source rank and expert after an AllToAll), a multiple of the experts, at most 1024, in any order but
     without overlap (segments that share rows leave every row of the result undefined); ``packed`` uint8
-    [experts, n, inner / 2] and ``scales`` [experts, n, inner / group] of the rows' dtype or float32, as :func:`quantize_int4` gives them, in groups of 32, 64 or 128.  Products and sums are
-    fp32, rounded once.  No gradients: 4-bit weights are for serving.  The kernel's waits are bounded: outputs whose
-    weights did not arrive in a second are NaN, and :func:`check_status` says so.
+    [experts, n, inner / 2] and ``scales`` [experts, n, inner / group] of the rows' dtype or float32, as
+    :func:`quantize_int4` gives them, in groups of 32, 64 or 128.  Products and sums are fp32, rounded once.  No
+    gradients: 4-bit weights are for serving.  The kernel's waits are bounded: outputs whose weights did not arrive
+    within a second of the GPU's timer are NaN, and :func:`check_status` says so.
     """
     return _call("int4_product", lambda: _check_product(rows, starts, counts, packed, scales, out), rows, starts, counts,
                  packed, scales, out, _GIVE_UP)
