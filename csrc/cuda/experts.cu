@@ -1,5 +1,7 @@
 // Mixture-of-experts operators on both sides of an AllToAll of tokens: the router's choice, the stable sort of
 // assignments by expert, the copy of tokens to their experts' rows and the weighted sum back, with gradients.
+//
+// Times compare forms on one set of inputs, launched again and again: inputs below 126 MB are then in the L2.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -558,7 +560,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) combine_kernel(ExchangeRowsArg
 // One CTA per token, its warps share the pieces: a piece of the gradient is read once and multiplied with and into
 // each of the token's rows.  The products of the pieces are added in a fixed order.  Many rows are held to 64
 // registers a thread for their warps' sake (8192 x 8 x 2048 bf16: 106 -> 98.5 us), few are faster without (256 x 8 x
-// 4096: 6.0 us, held 6.8).
+// 4096: 6.0 us, held 6.8).  Many are those that are streamed; where between the two sizes the forms meet was not measured.
 template <typename T, int N, bool STREAM>
 __global__ void __launch_bounds__(kRowWarps * 32, STREAM ? 4 : 1) combine_backward_kernel(ExchangeRowsArgs a, long long units, unsigned clear_blocks) {
   using V = Vec<T, N>;

@@ -14,12 +14,13 @@
 // fragment is one conflict-free 16-byte load.  A cluster of 1 to 8 CTAs splits the inner size where the CTAs would
 // not fill the GPU and joins its fp32 sums through distributed shared memory in the order of the CTAs.
 //
-// One row for each of 8 experts 4096 x 4096 (69 MB): 20.6 us, 3.3 TB/s.  The same kernel takes 15 us without its
-// arithmetic and 14 without its loads, so what is left is that the two overlap only in part: the arithmetic keeps
-// its integer pipe 60 % busy, and 16 warps of an SM are what its registers and ring allow.  Measured and not kept:
-// three CTAs of fewer registers (24.5 us), a barrier per 2 KB box (22.8), and one CTA per SM walking equal runs of
-// strips (26.8).  From about 16 rows an expert on the matrix unit bounds it: 1024 rows of 8 experts 1024 x 2048 take
-// 30.9 us, 139 TFLOP/s.
+// Times are of launches in a graph on inputs that are not in the L2, unless they say otherwise.  One row for each of 8
+// experts 4096 x 4096 (69 MB): 20.5 us, 3.4 TB/s.  With these inputs in the L2 it takes 18.0, without its arithmetic 15
+// and without its loads 14, so what is left is that the two overlap only in part: the arithmetic keeps its integer pipe
+// 60 % busy, and 16 warps of an SM are what its registers and ring allow.  Measured as calls and not kept, where this
+// form took 20.2 to 20.6: three CTAs of fewer registers (24.5), a barrier per 2 KB box (22.8), and one CTA per SM
+// walking equal runs of strips (26.8).  From about 16 rows an expert on the matrix unit bounds it: 1024 rows of 8
+// experts 1024 x 2048 take 30.1 us, 143 TFLOP/s.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -42,11 +43,12 @@ constexpr int kBoxes = 2;             // boxes of a tile
 constexpr int kTileK = kBoxes * kBoxK;
 constexpr int kStages = 2;            // tiles in flight of a warp
 constexpr unsigned kBoxBytes = 16 * 128;
+constexpr int kSms = 148;             // of a B200
 constexpr int kPool = 44 * 1024;      // shared memory for a stage of x and scales
 constexpr unsigned kTileBytes = kBoxes * kBoxBytes;
 constexpr unsigned kFull = 0xffffffffu;
-constexpr unsigned kWaitNs = 1000000000u;   // of a tile, and of what is in flight once a tile did not come; a limit
-                                            // from the arguments costs a register: ragged fp16 rows 16.7 -> 17.3 us
+constexpr unsigned kWaitNs = 1000000000u;   // of a tile, and of what is in flight once a tile did not come; a limit from the
+                                            // arguments costs a register (ragged fp16 rows in the L2 16.7 -> 17.3 us)
 
 // set when a copy did not arrive in time: the outputs it was for are NaN
 __device__ int late_copies = 0;
@@ -59,9 +61,10 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
 
 // q - 8 of the 4-bit values at bits [0, 4) (HIGH 0) or [4, 8) (HIGH 1) of both halves of w, in two instructions.
-// fp16: 1024 + q (or 1024 + 16 q) has q in its mantissa, and one fma takes the 1024 off.  bf16 has too few mantissa
-// bits for the upper four, but below 2^-125 its numbers are evenly spaced, so the masked bits are already q 2^-133
-// or 16 q 2^-133; one fma makes them (q - 8) 2^-6, and the total is multiplied by 64 once at the end.  All exact.
+// fp16: 1024 + q (or 1024 + 16 q) has q in its mantissa, and one fma takes the 1024 off (the published way to read small
+// integers as floats: Kim, Henry, Fahim, Awadalla, Who Says Elephants Can't Run, 2022).  bf16 has too few mantissa bits
+// for the upper four, but below 2^-125 its numbers are evenly spaced, so the masked bits are already q 2^-133 or
+// 16 q 2^-133; one fma makes them (q - 8) 2^-6, and the total is multiplied by 64 once at the end.  All exact.
 template <typename T, int HIGH>
 __device__ __forceinline__ unsigned two_values(unsigned w) {
   constexpr unsigned mask = HIGH ? 0x00f000f0u : 0x000f000fu;
@@ -356,7 +359,7 @@ __device__ __forceinline__ void item_sums(const CUtensorMap* map, const Int4Args
         if (late < 0 && !__all_sync(kFull, wait_tile(bar + 8 * slot, phase))) late = (c0 + u0) / UNITS;
         const unsigned char* tile = ring + slot * kTileBytes;
         if (u0 + UNITS <= here) {
-          // unrolled with one column only: with more the registers spill (1024 rows of 8 experts 32.7 us, so 28.8)
+          // unrolled with one column only: with more the registers spill (1024 rows of 8 experts 34.9 us, so 30.1)
 #pragma unroll (COLS == 1 ? UNITS : 1)
           for (int u = 0; u < UNITS; u += PAIR)
             group_product<T, S, VEC, COLS, PAIR>(acc, tile, lane_at, u, xw + u * VEC * step, step, sw + u, 8 * pitch);
@@ -516,7 +519,7 @@ cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
   const long long n_tiles = (a.n + kTileN - 1) / kTileN;
   // split the inner size until the GPU is full, as long as a CTA keeps a tile
   int ranks = 1;
-  while (ranks < 8 && n_tiles * items * ranks * 2 <= 148 * 2 && a.inner / (2 * ranks) >= kTileK) ranks *= 2;
+  while (ranks < 8 && n_tiles * items * ranks * 2 <= kSms * 2 && a.inner / (2 * ranks) >= kTileK) ranks *= 2;
   Geometry geo{};
   const long long tiles = (a.inner + kTileK - 1) / kTileK;
   geo.slice = (tiles + ranks - 1) / ranks * kTileK;
@@ -558,7 +561,8 @@ cudaError_t launch(const Int4Args& a, cudaStream_t stream) {
   return cudaLaunchKernelEx(&config, kernel, map, a, geo);
 }
 
-// up to 8 rows have one column: an instance without the others' registers (one token of 8 experts 19.3 us, not 20.4)
+// Up to 8 rows have one column: an instance without the others' registers (one token of 8 experts 20.5 us, not 21.3).
+// The host knows only the rows of the call, so more rows take the other instance however few each expert has.
 template <typename T, typename S, int VEC>
 cudaError_t launch_columns(const Int4Args& a, cudaStream_t stream) {
   return a.rows <= 8 ? launch<T, S, VEC, 1>(a, stream) : launch<T, S, VEC, 4>(a, stream);
