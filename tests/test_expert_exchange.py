@@ -325,3 +325,22 @@ def test_explicit_gradients_are_handed_on_by_the_caller():
     want = ex.combine(ex.dispatch(x2 * 3, order) * 2, w2, order)
     want.backward(grad)
     assert torch.equal(out, want) and torch.equal(x.grad, x2.grad) and torch.equal(l.grad, l2.grad)
+
+
+@pytest.mark.gpu
+def test_products_of_another_number_of_experts_and_foreign_rows_are_refused():
+    gpu()
+    exchange = alone(experts=4, hidden=64, capacity=3)
+    x, logits, _ = tokens_for(0, 4, 4, 1, 64, torch.bfloat16)
+    ids, w = ex.route(logits, 1)
+    packed, scales = ex.quantize_int4(torch.ones(5, 64, 64, device="cuda").bfloat16(), 32)
+    with pytest.raises(RuntimeFailure, match="first"):
+        exchange.matmul_int4(x, packed[:4], scales[:4])
+    rows = exchange.dispatch(x, ids)
+    for count in (3, 5):
+        with pytest.raises(RuntimeFailure, match="experts"):
+            exchange.matmul_int4(rows, packed[:count], scales[:count])
+    assert exchange.matmul_int4(rows, packed[:4], scales[:4]).shape == (12, 64)
+    for wrong in (rows[:11], rows[:, :63], rows.float()):
+        with pytest.raises(RuntimeFailure, match="rows"):
+            exchange.combine(wrong, w)
